@@ -96,7 +96,8 @@ typedef enum dcn_status {
 
 typedef enum dcn_dtype {
     DCN_DTYPE_F32 = 0,
-    DCN_DTYPE_F16 = 1
+    DCN_DTYPE_F16 = 1,
+    DCN_DTYPE_BF16 = 2        /* token operators only */
 } dcn_dtype;
 
 typedef enum dcn_weight_layout {
@@ -421,6 +422,145 @@ dcn_status dcn_forward_f16_static_scratch(const dcn_shape *shape, const void *in
                                           const void *packed_weight, const void *bias,
                                           void *output, uint32_t *nonfinite_flag,
                                           dcn_stream stream);
+
+/* ---- token operators ------------------------------------------------------------
+ * A transformer block over the tokens of a tile stream, next to the convolution: tokens are
+ * patches of a tile's features, frame after frame, and a new frame's tokens attend to the frames
+ * that the stream keeps in a paged cache.  No counterpart in the reference, whose network carries
+ * information between frames by flow and convolution only.  Everything but the block's matrix
+ * products is here: the position rotation, the cache append, the attention over the cache, and
+ * the norms before and after the block with its gate and residual.
+ *
+ * Tensors may be strided: a token tensor is [tokens][heads][head_dim] with the strides of dcn_heads
+ * (in elements) and unit stride along head_dim.  A token count of zero is a valid call that
+ * launches nothing.  Arithmetic is FP32 whatever the element type, rounded once per output. */
+
+/* A strided [tokens][heads][head_dim] tensor (strides in elements, non-negative). */
+typedef struct dcn_heads {
+    void *data;
+    int64_t token_stride;
+    int64_t head_stride;
+} dcn_heads;
+
+/* Rotary positions over three axes (time, row, column).  Pair j of a head belongs to axis 0 for
+ * j < pairs[0], to axis 1 for the next pairs[1] and to axis 2 for the last pairs[2]; token t turns
+ * it by positions[t][axis] * frequencies[j] radians:
+ *   (a, b) -> (a cos - b sin, a sin + b cos).
+ * interleaved != 0: pair j is elements (2j, 2j+1); 0: elements (j, j + P), P = pairs[0] + pairs[1]
+ * + pairs[2] <= head_dim / 2.  Elements from 2P on stay as they are.  Angles are formed and reduced
+ * in FP64, so they stay exact to FP32 for any int32 position. */
+typedef struct dcn_rotation {
+    const double *frequencies; /* [P] */
+    const int32_t *positions;  /* [tokens][3] */
+    int32_t pairs[3];
+    int32_t interleaved;
+} dcn_rotation;
+
+/* A paged key/value cache and the streams that live in it.
+ *   keys, values   [pages][page_size][heads][head_dim], unit stride along head_dim, the other
+ *                  strides in elements (a contiguous [streams][capacity] cache is the case
+ *                  page_size = capacity)
+ *   table          [streams][table_columns] page ids (row stride table_stride): position p of
+ *                  stream b lies in page table[b][p / page_size], slot p % page_size
+ *   starts         [streams + 1]: stream b's tokens of this step are [starts[b], starts[b + 1])
+ *   lengths        [streams]: tokens of stream b, this step's included, so the i-th of its n
+ *                  tokens of this step is at position lengths[b] - n + i
+ * table, starts and lengths are read on the device.  Positions outside the table and page ids
+ * outside [0, pages) are never accessed: an append there writes nothing, an attention reads such a
+ * key and value as zeros. */
+typedef struct dcn_paged_cache {
+    void *keys;
+    void *values;
+    int64_t key_page_stride, key_slot_stride, key_head_stride;
+    int64_t value_page_stride, value_slot_stride, value_head_stride;
+    int32_t pages, page_size, heads, head_dim;
+    int32_t dtype; /* dcn_dtype */
+    int32_t streams, table_columns;
+    int32_t reserved; /* 0 */
+    int64_t table_stride;
+    const int32_t *table;
+    const int32_t *starts;
+    const int32_t *lengths;
+} dcn_paged_cache;
+
+/* Rotates x into out (which may be x itself).  Any dtype; head_dim even, at most 512. */
+dcn_status dcn_token_rotary(dcn_dtype dtype, int64_t tokens, int32_t heads, int32_t head_dim,
+                            const dcn_rotation *rotation, const dcn_heads *x, const dcn_heads *out,
+                            dcn_stream stream);
+
+/* Appends a step's keys and values to the cache, and rotates its queries in the same launch: keys
+ * are rotated and stored at their stream's positions, values are stored as they are, queries
+ * (nullable: q_heads 0 and q, q_out NULL) are rotated into q_out (which may be q).  rotation NULL
+ * stores keys as they are.  `tokens` is the token tensors' extent; tokens at or past
+ * starts[streams] and tokens at a negative position are not stored. */
+dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const dcn_rotation *rotation,
+                            const dcn_heads *keys, const dcn_heads *values, int32_t q_heads,
+                            const dcn_heads *q, const dcn_heads *q_out, dcn_stream stream);
+
+/* Attention of a step's queries over the cache.  A frame is `frame` consecutive positions of a
+ * stream (1: every token its own).  The query at position p sees the key at position s < length when
+ *   s/frame <= p/frame, and  s/frame > p/frame - window  or  s/frame < sinks
+ * (tokens of one frame see each other; the last `window` frames and the first `sinks` frames are
+ * visible).  out = softmax(scale * q.k) v over the visible keys, zeros where there are none.  What
+ * hidden keys and values hold, non-finite values included, does not reach the result.
+ * q_heads is a multiple of the cache's heads: query head h reads key head h / (q_heads / heads).
+ *   max_q    at least the longest step starts[b + 1] - starts[b]
+ *   max_kv   at least the largest length (it sizes the split over keys; a longer stream is
+ *            still computed in full)
+ * FP16 and BF16 with head_dim 64 or 128, 16-byte aligned tensors and strides, page_size a multiple
+ * of 16 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
+ * 256, other strides) on CUDA cores.  `workspace` holds
+ * dcn_token_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0). */
+typedef struct dcn_token_attention_args {
+    int64_t tokens; /* rows of q and out */
+    int32_t q_heads;
+    int32_t max_q;
+    int32_t max_kv;
+    int32_t window; /* >= 1 */
+    int32_t sinks;  /* >= 0 */
+    int32_t frame;  /* >= 1 */
+    float scale;
+    int32_t reserved; /* 0 */
+} dcn_token_attention_args;
+
+size_t dcn_token_attention_workspace_bytes(const dcn_paged_cache *cache, const dcn_token_attention_args *args);
+dcn_status dcn_token_attention(const dcn_paged_cache *cache, const dcn_token_attention_args *args,
+                               const dcn_heads *q, const dcn_heads *out, void *workspace,
+                               size_t workspace_bytes, dcn_stream stream);
+
+/* The norms around a block.  Per row of `width` elements, with g = row / group the row's modulation
+ * group:
+ *   branch = post ? N(x) * post_weight + post_bias : x
+ *   hidden = residual ? residual_scale * residual + gate[g] * branch : x       -> hidden (nullable)
+ *   y      = N(hidden) * weight + bias
+ *   out    = y * (1 + scale[g]) + shift[g]
+ * N is x / sqrt(mean(x^2) + epsilon) or (x - mean) / sqrt(var + epsilon).  Every vector may be NULL
+ * (weights 1, biases 0, gate 1, scale and shift 0); post, gate and hidden need a residual.  N(hidden)
+ * takes the FP32 hidden, before its rounding to the element type.  Row strides are in elements;
+ * width up to 8192.  hidden may be residual or x itself, out may be x. */
+typedef enum dcn_norm_kind {
+    DCN_NORM_RMS = 0,
+    DCN_NORM_LAYER = 1
+} dcn_norm_kind;
+
+typedef struct dcn_token_norm_args {
+    int64_t rows;
+    int64_t group; /* >= 1 */
+    int32_t width;
+    int32_t dtype; /* dcn_dtype */
+    int32_t kind;  /* dcn_norm_kind */
+    int32_t post;  /* 1: normalise x before the gate */
+    float epsilon;
+    float residual_scale;
+    const void *x, *residual;
+    const void *post_weight, *post_bias, *weight, *bias; /* [width] */
+    const void *gate, *scale, *shift;                    /* [groups][width] */
+    void *hidden, *out;
+    int64_t x_stride, residual_stride, hidden_stride, out_stride;
+    int64_t gate_stride, scale_stride, shift_stride;
+} dcn_token_norm_args;
+
+dcn_status dcn_token_norm(const dcn_token_norm_args *args, dcn_stream stream);
 
 /* ---- device error word ----------------------------------------------------------
  * Every kernel with a bounded device-side wait records a timeout in a sticky

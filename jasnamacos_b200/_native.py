@@ -27,6 +27,10 @@ DCN_ERR_SCRATCH_TOO_SMALL = 9
 
 DCN_DTYPE_F32 = 0
 DCN_DTYPE_F16 = 1
+DCN_DTYPE_BF16 = 2
+
+DCN_NORM_RMS = 0
+DCN_NORM_LAYER = 1
 
 DCN_WEIGHT_OIHW = 0
 DCN_WEIGHT_IC_K_OC = 1
@@ -94,7 +98,72 @@ class DcnPlan(ctypes.Structure):
     ]
 
 
+class DcnHeads(ctypes.Structure):
+    """`struct dcn_heads`: a strided [tokens][heads][head_dim] tensor."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class DcnRotation(ctypes.Structure):
+    """`struct dcn_rotation`: rotary positions over three axes."""
+
+    _fields_ = [
+        ("frequencies", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32 * 3),
+        ("interleaved", ctypes.c_int32),
+    ]
+
+
+class DcnPagedCache(ctypes.Structure):
+    """`struct dcn_paged_cache`: a paged key/value cache and the streams in it."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        *[(name, ctypes.c_int64) for name in ("key_page_stride", "key_slot_stride", "key_head_stride",
+                                              "value_page_stride", "value_slot_stride", "value_head_stride")],
+        *[(name, ctypes.c_int32) for name in ("pages", "page_size", "heads", "head_dim", "dtype", "streams",
+                                              "table_columns", "reserved")],
+        ("table_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class DcnTokenAttentionArgs(ctypes.Structure):
+    """`struct dcn_token_attention_args`."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        *[(name, ctypes.c_int32) for name in ("q_heads", "max_q", "max_kv", "window", "sinks", "frame")],
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class DcnTokenNormArgs(ctypes.Structure):
+    """`struct dcn_token_norm_args`."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("group", ctypes.c_int64),
+        *[(name, ctypes.c_int32) for name in ("width", "dtype", "kind", "post")],
+        ("epsilon", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+        *[(name, ctypes.c_void_p) for name in ("x", "residual", "post_weight", "post_bias", "weight", "bias",
+                                               "gate", "scale", "shift", "hidden", "out")],
+        *[(name, ctypes.c_int64) for name in ("x_stride", "residual_stride", "hidden_stride", "out_stride",
+                                              "gate_stride", "scale_stride", "shift_stride")],
+    ]
+
+
 _P = ctypes.c_void_p
+_HEADS = ctypes.POINTER(DcnHeads)
+_ROTATION = ctypes.POINTER(DcnRotation)
+_CACHE = ctypes.POINTER(DcnPagedCache)
+_ATTENTION = ctypes.POINTER(DcnTokenAttentionArgs)
 _SHAPE = ctypes.POINTER(DcnShape)
 _IO = ctypes.POINTER(DcnIo)
 
@@ -147,6 +216,13 @@ PROTOTYPES = {
     "dcn_temporal_slabs_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     "dcn_temporal_prepare_slabs_f16": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P,
                                                       _P, ctypes.c_int32, _P, _P, _P, ctypes.c_size_t, _P]),
+    "dcn_token_rotary": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _ROTATION,
+                                        _HEADS, _HEADS, _P]),
+    "dcn_token_append": (ctypes.c_int, [_CACHE, ctypes.c_int64, _ROTATION, _HEADS, _HEADS, ctypes.c_int32, _HEADS,
+                                        _HEADS, _P]),
+    "dcn_token_attention_workspace_bytes": (ctypes.c_size_t, [_CACHE, _ATTENTION]),
+    "dcn_token_attention": (ctypes.c_int, [_CACHE, _ATTENTION, _HEADS, _HEADS, _P, ctypes.c_size_t, _P]),
+    "dcn_token_norm": (ctypes.c_int, [ctypes.POINTER(DcnTokenNormArgs), _P]),
     "dcn_device_error": (ctypes.c_int, []),
     "dcn_check_wait_timeout": (ctypes.c_int, [ctypes.c_uint32, _P]),
     "dcn_forward_f16_host_workspace_bytes": (ctypes.c_size_t, [_SHAPE, ctypes.c_int32]),

@@ -34,8 +34,12 @@ SOURCES = [
     "dcn_host.cu",
     "dcn_temporal.cu",
     "dcn_nhwc.cu",
+    "dcn_token_api.cu",
+    "dcn_token_norm.cu",
+    "dcn_token_rotary.cu",
+    "dcn_token_attention.cu",
 ]
-HEADERS = ["dcn_common.cuh"]
+HEADERS = ["dcn_common.cuh", "dcn_tokens.cuh", "dcn_token_attention.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -216,6 +216,16 @@ dcn_path select_path(const Params &p) {
 }
 
 }  // namespace
+
+dcn_status launch_device(LaunchDevice *out) {
+    DeviceInfo *d = nullptr;
+    const dcn_status st = current_device(&d);
+    if (st == DCN_OK) *out = LaunchDevice{d->sm_count, d->err_word};
+    return st;
+}
+
+dcn_status status_from_cuda(cudaError_t e) { return from_cuda(e); }
+
 }  // namespace dcn
 
 using namespace dcn;

@@ -72,6 +72,14 @@ struct SplitInput {
 // runtime creates a new primary context, in which the old addresses are meaningless.
 uint64_t current_context_id();
 
+// What a launch needs to know of the current device; set up once per device and context.
+struct LaunchDevice {
+    int sm_count;
+    uint32_t *err_word;
+};
+dcn_status launch_device(LaunchDevice *out);
+dcn_status status_from_cuda(cudaError_t e);
+
 // Longest any device-side wait may spin before it gives up and reports
 // DCN_ERR_DEVICE_TIMEOUT (nanoseconds of %globaltimer).
 constexpr uint64_t kWaitLimitNs = 2000000000ull;

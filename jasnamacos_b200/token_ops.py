@@ -1,0 +1,307 @@
+"""Token operators: a streaming transformer block next to the deformable convolution.
+
+Tokens are patches of a tile's features, frame after frame.  A block over them is library matrix
+products plus the four operators here (``dcn_token_*`` of ``include/dcn_b200.h``):
+
+* :meth:`CudaTokenOps.norm`, :meth:`CudaTokenOps.residual_norm` -- the norms before and after a block,
+  with its gate, residual scale and modulation
+* :meth:`CudaTokenOps.rotary` -- rotary positions over (time, row, column)
+* :meth:`CudaTokenOps.append` -- a step's keys and values into a paged cache, rotated on the way,
+  and its queries rotated with them
+* :meth:`CudaTokenOps.attention` -- the step's queries over the cache: the last ``window`` frames and
+  the first ``sinks`` frames
+
+The reference has no counterpart: its network carries information between frames by flow and
+convolution only.  Everything computes in ``libdcn_b200.so``; PyTorch provides device memory and
+streams.  There is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native
+from .deform_conv import DeviceUnavailable, InvalidArgument, raise_for_status
+
+_DTYPES = {torch.float32: _native.DCN_DTYPE_F32, torch.float16: _native.DCN_DTYPE_F16,
+           torch.bfloat16: _native.DCN_DTYPE_BF16}
+_KINDS = {"rms": _native.DCN_NORM_RMS, "layer": _native.DCN_NORM_LAYER}
+
+
+def _heads(t) -> _native.DcnHeads:
+    stride = t.stride()
+    return _native.DcnHeads(t.data_ptr(), stride[0], stride[1])
+
+
+class CudaTokenOps:
+    """The token operators on CUDA tensors.
+
+    Methods enqueue on the current stream of the tensors' device, or on ``stream``, and return without
+    waiting.  Token tensors are ``[tokens, heads, head_dim]`` with any strides but a unit one along
+    ``head_dim``; results are new tensors unless ``out`` is given.
+    """
+
+    def __init__(self, device: int | None = None):
+        self.lib = _native.load()
+        if not torch.cuda.is_available():
+            raise DeviceUnavailable()
+        self.device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
+
+    # -- checks ------------------------------------------------------------------
+    def _dtype(self, t) -> int:
+        dtype = _DTYPES.get(t.dtype)
+        if dtype is None:
+            raise InvalidArgument(f"element type {t.dtype}: float32, float16 or bfloat16 is wanted")
+        return dtype
+
+    def _tokens(self, name, t, tokens, heads, head_dim, dtype) -> None:
+        """A [tokens][heads][head_dim] tensor with unit stride along head_dim on this device."""
+        if t.shape != (tokens, heads, head_dim) or t.dtype != dtype or t.device != self.device:
+            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; "
+                                  f"({tokens}, {heads}, {head_dim}) {dtype} on {self.device} is wanted")
+        if t.stride(2) != 1 and head_dim > 1:
+            raise InvalidArgument(f"{name} needs unit stride along its last dimension")
+
+    def _whole(self, name, t, shape, dtype) -> None:
+        """A contiguous tensor of a given shape and type on this device."""
+        if t.shape != shape or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
+            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; a contiguous {tuple(shape)} "
+                                  f"{dtype} tensor on {self.device} is wanted")
+
+    def _call(self, stream, function, *args) -> None:
+        """Calls the library on this operator's device and the given or current stream."""
+        index = self.device.index
+        handle = torch.cuda.current_stream(index).cuda_stream if stream is None else stream.cuda_stream
+        if torch.cuda.current_device() == index:
+            status = function(*args, handle or None)
+        else:
+            with torch.cuda.device(index):
+                status = function(*args, handle or None)
+        if status != _native.DCN_OK:
+            raise_for_status(status, function.__name__)
+
+    def _rotation(self, positions, frequencies, pairs, interleaved, tokens) -> _native.DcnRotation:
+        pairs = tuple(pairs)
+        if len(pairs) != 3 or min(pairs) < 0:
+            raise InvalidArgument(f"pairs {pairs}: one count for each of three axes is wanted")
+        self._whole("positions", positions, (tokens, 3), torch.int32)
+        self._whole("frequencies", frequencies, (sum(pairs),), torch.float64)
+        return _native.DcnRotation(frequencies.data_ptr(), positions.data_ptr(), pairs, bool(interleaved))
+
+    def _cache(self, k_cache, v_cache, table, starts, lengths) -> _native.DcnPagedCache:
+        if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+            raise InvalidArgument(f"k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
+                                  f"{v_cache.dtype}: two [pages, page_size, heads, head_dim] tensors of one type are wanted")
+        pages, page_size, heads, head_dim = k_cache.shape
+        ks, vs = k_cache.stride(), v_cache.stride()
+        if k_cache.device != self.device or v_cache.device != self.device or ks[3] != 1 or vs[3] != 1:
+            raise InvalidArgument(f"k_cache and v_cache need unit stride along head_dim and to be on {self.device}")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or table.stride(1) != 1:
+            raise InvalidArgument(f"table: a [streams, columns] int32 tensor on {self.device} is wanted")
+        streams, columns = table.shape
+        self._whole("starts", starts, (streams + 1,), torch.int32)
+        self._whole("lengths", lengths, (streams,), torch.int32)
+        return _native.DcnPagedCache(
+            k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, page_size, heads,
+            head_dim, self._dtype(k_cache), streams, columns, 0, table.stride(0), table.data_ptr(), starts.data_ptr(),
+            lengths.data_ptr())
+
+    # -- positions and cache -----------------------------------------------------
+    def rotary(self, x, positions, frequencies, pairs, interleaved=False, out=None, stream=None):
+        """Rotates the heads of `x` [tokens, heads, head_dim] by their token's position.
+
+        Pair j belongs to axis 0 (time) for j < pairs[0], then to axis 1 (row) for pairs[1] pairs and to
+        axis 2 (column) for pairs[2]; it turns by ``positions[token, axis] * frequencies[j]`` radians.
+        `positions` is int32 [tokens, 3], `frequencies` float64 [sum(pairs)].  Pairs are elements
+        (2j, 2j+1) when `interleaved`, else (j, j + sum(pairs)); elements past them stay.  `out` may be `x`."""
+        if x.dim() != 3:
+            raise InvalidArgument(f"x is {tuple(x.shape)}; [tokens, heads, head_dim] is wanted")
+        if stream is not None and out is None:
+            with torch.cuda.stream(stream):  # the result belongs to the stream that writes it
+                out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        tokens, heads, head_dim = x.shape
+        self._tokens("x", x, tokens, heads, head_dim, x.dtype)
+        rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
+        if out is None:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        else:
+            self._tokens("out", out, tokens, heads, head_dim, x.dtype)
+        self._call(stream, self.lib.dcn_token_rotary, self._dtype(x), tokens, heads, head_dim, rotation, _heads(x),
+                   _heads(out))
+        return out
+
+    def append(self, k, v, k_cache, v_cache, table, starts, lengths, q=None, positions=None, frequencies=None,
+               pairs=(0, 0, 0), interleaved=False, q_out=None, stream=None):
+        """Writes a step's keys and values into the cache and rotates its queries, in one launch.
+
+        `k`, `v` [tokens, kv_heads, head_dim]; stream b's tokens are [starts[b], starts[b+1]) and end at
+        position lengths[b] - 1 (lengths count this step).  Position p lies in page table[b, p // page_size]
+        of `k_cache`, `v_cache` [pages, page_size, kv_heads, head_dim].  With `positions`, keys and the
+        queries `q` [tokens, q_heads, head_dim] are rotated as :meth:`rotary` does.  Returns the rotated
+        queries (`q_out`, which may be `q`), or None without `q`."""
+        cache = self._cache(k_cache, v_cache, table, starts, lengths)
+        if k.dim() != 3:
+            raise InvalidArgument(f"k is {tuple(k.shape)}; [tokens, kv_heads, head_dim] is wanted")
+        tokens, dtype = k.shape[0], k_cache.dtype
+        self._tokens("k", k, tokens, cache.heads, cache.head_dim, dtype)
+        self._tokens("v", v, tokens, cache.heads, cache.head_dim, dtype)
+        rotation = None
+        if positions is not None:
+            rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
+        elif frequencies is not None or any(pairs):
+            raise InvalidArgument("a rotation needs positions")
+        q_heads, q_from, q_to = 0, None, None
+        if q is not None:
+            if q.dim() != 3:
+                raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
+            q_heads = q.shape[1]
+            self._tokens("q", q, tokens, q_heads, cache.head_dim, dtype)
+            if q_out is None:
+                if stream is None:
+                    q_out = torch.empty(q.shape, dtype=dtype, device=self.device)
+                else:
+                    with torch.cuda.stream(stream):
+                        q_out = torch.empty(q.shape, dtype=dtype, device=self.device)
+            else:
+                self._tokens("q_out", q_out, tokens, q_heads, cache.head_dim, dtype)
+            q_from, q_to = _heads(q), _heads(q_out)
+        elif q_out is not None:
+            raise InvalidArgument("q_out needs q")
+        self._call(stream, self.lib.dcn_token_append, cache, tokens, rotation, _heads(k), _heads(v), q_heads, q_from, q_to)
+        return q_out
+
+    # -- attention ---------------------------------------------------------------
+    def attention(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0, frame=1, scale=None,
+                  out=None, workspace=None, stream=None):
+        """Attention of a step's queries `q` [tokens, q_heads, head_dim] over the cache of :meth:`append`.
+
+        A frame is `frame` consecutive positions.  A query sees its own frame and those before it in the
+        stream, of these the last `window` frames and the first `sinks` frames; frame = 1 is plain causal
+        attention with a sliding window and first tokens that stay.  `max_q` bounds the streams' steps and
+        `max_kv` their lengths.  `scale` defaults to head_dim ** -0.5.  A query that sees no key gives zeros.
+        `workspace` (uint8, :meth:`attention_workspace_bytes`) is taken from PyTorch when not given."""
+        if q.dim() != 3:
+            raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
+        cache = self._cache(k_cache, v_cache, table, starts, lengths)
+        tokens, q_heads, head_dim = q.shape
+        self._tokens("q", q, tokens, q_heads, cache.head_dim, k_cache.dtype)
+        args = _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame,
+                                             1.0 / math.sqrt(head_dim) if scale is None else scale, 0)
+        if out is not None:
+            self._tokens("out", out, tokens, q_heads, head_dim, q.dtype)
+        need = self.lib.dcn_token_attention_workspace_bytes(cache, args)
+        if stream is None or (out is not None and (workspace is not None or need == 0)):
+            return self._attention(cache, args, q, out, workspace, need, stream)
+        with torch.cuda.stream(stream):
+            return self._attention(cache, args, q, out, workspace, need, stream)
+
+    def _attention(self, cache, args, q, out, workspace, need, stream):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        given = 0
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        if workspace is not None:
+            if workspace.device != self.device or not workspace.is_contiguous():
+                raise InvalidArgument(f"workspace: contiguous memory on {self.device} is wanted")
+            given = workspace.numel() * workspace.element_size()
+        self._call(stream, self.lib.dcn_token_attention, cache, args, _heads(q), _heads(out),
+                   None if workspace is None else workspace.data_ptr(), given)
+        return out
+
+    def attention_workspace_bytes(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0,
+                                  frame=1) -> int:
+        """Bytes of scratch that :meth:`attention` takes for these tensors."""
+        cache = self._cache(k_cache, v_cache, table, starts, lengths)
+        args = _native.DcnTokenAttentionArgs(q.shape[0], q.shape[1], max_q, max_kv, window, sinks, frame, 1.0, 0)
+        return int(self.lib.dcn_token_attention_workspace_bytes(cache, args))
+
+    # -- norms -------------------------------------------------------------------
+    def _vector(self, name, t, width, dtype):
+        if t is None:
+            return None
+        self._whole(name, t, (width,), dtype)
+        return t.data_ptr()
+
+    def _modulation(self, name, t, groups, width, dtype):
+        """Pointer and row stride of a [groups, width] tensor with unit stride along its rows."""
+        if t is None:
+            return None, 0
+        if t.dim() != 2 or t.shape[0] < groups or t.shape[1] != width or t.dtype != dtype or t.device != self.device or \
+                (t.stride(1) != 1 and width > 1):
+            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; [{groups}, {width}] {dtype} with unit "
+                                  f"stride along its rows on {self.device} is wanted")
+        return t.data_ptr(), t.stride(0)
+
+    def _rows(self, name, t, shape, dtype) -> int:
+        if t.shape != shape or t.dtype != dtype or t.device != self.device or (t.stride(1) != 1 and shape[1] > 1):
+            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; {tuple(shape)} {dtype} with unit stride "
+                                  f"along its rows on {self.device} is wanted")
+        return t.stride(0)
+
+    def _norm(self, x, residual, post, post_weight, post_bias, gate, residual_scale, kind, weight, bias, scale, shift, group,
+              eps, hidden, out, stream):
+        if x.dim() != 2:
+            raise InvalidArgument(f"x is {tuple(x.shape)}; [rows, width] is wanted")
+        shape, dtype = x.shape, x.dtype
+        rows, width = shape
+        if kind not in _KINDS:
+            raise InvalidArgument(f"kind {kind!r}: 'rms' or 'layer' is wanted")
+        if group is None:
+            group = max(1, rows)
+        if group < 1:
+            raise InvalidArgument(f"group {group}: at least one row shares a modulation row")
+        groups = -(-rows // group)
+        gate_at, gate_stride = self._modulation("gate", gate, groups, width, dtype)
+        scale_at, scale_stride = self._modulation("scale", scale, groups, width, dtype)
+        shift_at, shift_stride = self._modulation("shift", shift, groups, width, dtype)
+        args = _native.DcnTokenNormArgs(
+            rows, group, width, self._dtype(x), _KINDS[kind], post, eps, residual_scale, x.data_ptr(),
+            None if residual is None else residual.data_ptr(), self._vector("post_weight", post_weight, width, dtype),
+            self._vector("post_bias", post_bias, width, dtype), self._vector("weight", weight, width, dtype),
+            self._vector("bias", bias, width, dtype), gate_at, scale_at, shift_at,
+            None if hidden is None else hidden.data_ptr(), out.data_ptr(), self._rows("x", x, shape, dtype),
+            0 if residual is None else self._rows("residual", residual, shape, dtype),
+            0 if hidden is None else self._rows("hidden", hidden, shape, dtype), self._rows("out", out, shape, dtype),
+            gate_stride, scale_stride, shift_stride)
+        self._call(stream, self.lib.dcn_token_norm, args)
+
+    @staticmethod
+    def _new(x, stream):
+        if stream is None:
+            return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+    def norm(self, x, kind="rms", weight=None, bias=None, scale=None, shift=None, group=None, eps=1e-6, out=None, stream=None):
+        """The norm before a block: ``(N(x) * weight + bias) * (1 + scale[g]) + shift[g]`` for the rows of
+        `x` [rows, width], g = row // group (`group` None: one modulation row for all).  `kind` "rms" or
+        "layer"; `scale`, `shift` [groups, width], rows of any stride; `out` may be `x`."""
+        if out is None:
+            out = self._new(x, stream)
+        self._norm(x, None, 0, None, None, None, 1.0, kind, weight, bias, scale, shift, group, eps, None, out, stream)
+        return out
+
+    def residual_norm(self, x, residual, gate=None, post_weight=None, post_bias=None, residual_scale=1.0, kind="rms",
+                      weight=None, bias=None, scale=None, shift=None, group=None, eps=1e-6, hidden=None, out=None, stream=None):
+        """A block's end and the next one's norm, in one pass over the rows:
+
+        ``hidden = residual_scale * residual + gate[g] * branch`` and
+        ``out = (N(hidden) * weight + bias) * (1 + scale[g]) + shift[g]``,
+
+        with branch = `x`, or ``N(x) * post_weight + post_bias`` when `post_weight` is given (the norm after
+        the block).  Returns (hidden, out); `hidden` may be `residual` or `x`, `out` may be `x`."""
+        if residual is None:
+            raise InvalidArgument("residual_norm needs a residual")
+        if post_bias is not None and post_weight is None:
+            raise InvalidArgument("post_bias needs post_weight")
+        if hidden is None:
+            hidden = self._new(x, stream)
+        if out is None:
+            out = self._new(x, stream)
+        self._norm(x, residual, int(post_weight is not None), post_weight, post_bias, gate, residual_scale, kind, weight, bias,
+                   scale, shift, group, eps, hidden, out, stream)
+        return hidden, out
