@@ -463,7 +463,7 @@ typedef struct dcn_rotation {
  *   table          [streams][table_columns] page ids (row stride table_stride): position p of
  *                  stream b lies in page table[b][p / page_size], slot p % page_size
  *   starts         [streams + 1]: stream b's tokens of this step are [starts[b], starts[b + 1])
- *   lengths        [streams]: tokens of stream b, this step's included, so the i-th of its n
+ *   lengths        [streams]: tokens of stream b (below 2^31 - 1024), this step's included, so the i-th of its n
  *                  tokens of this step is at position lengths[b] - n + i
  * table, starts and lengths are read on the device.  Positions outside the table and page ids
  * outside [0, pages) are never accessed: an append there writes nothing, an attention reads such a
@@ -508,7 +508,7 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
  *   max_kv   at least the largest length (it sizes the split over keys; a longer stream is
  *            still computed in full)
  * FP16 and BF16 with head_dim 64 or 128, 16-byte aligned tensors and strides, page_size a multiple
- * of 16 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
+ * of 8 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
  * 256, other strides) on CUDA cores.  `workspace` holds
  * dcn_token_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0). */
 typedef struct dcn_token_attention_args {

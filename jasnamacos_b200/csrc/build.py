@@ -38,6 +38,7 @@ SOURCES = [
     "dcn_token_norm.cu",
     "dcn_token_rotary.cu",
     "dcn_token_attention.cu",
+    "dcn_token_attention_sm100.cu",
 ]
 HEADERS = ["dcn_common.cuh", "dcn_tokens.cuh", "dcn_token_attention.cuh"]
 
@@ -69,6 +70,8 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
         nvcc_path(),
         *ARCH_FLAGS,
         "-O3",
+        "--threads",
+        "0",
         "-lineinfo",
         "-std=c++17",
         "-Xcompiler",

@@ -74,6 +74,11 @@ dcn_status check_attention(const dcn_paged_cache *c, const dcn_token_attention_a
     return DCN_OK;
 }
 
+// Whether a 16-bit tensor's rows start on 16 bytes.
+bool packs(const dcn_heads &h) {
+    return aligned_to(h.data, 16) && h.token_stride % 8 == 0 && h.head_stride % 8 == 0;
+}
+
 HeadCopy copy_of(const dcn_heads &src, const dcn_heads &dst, int32_t heads, bool rotate) {
     HeadCopy c{};
     c.src = src.data;
@@ -166,8 +171,8 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
 }
 
 size_t dcn_token_attention_workspace_bytes(const dcn_paged_cache *cache, const dcn_token_attention_args *args) {
-    if (check_attention(cache, args) != DCN_OK) return 0;
-    return 0;
+    if (check_attention(cache, args) != DCN_OK || !token_attention_tensor(*cache, *args)) return 0;
+    return token_attention_tensor_workspace(*cache, *args);
 }
 
 dcn_status dcn_token_attention(const dcn_paged_cache *cache, const dcn_token_attention_args *args, const dcn_heads *q,
@@ -183,6 +188,9 @@ dcn_status dcn_token_attention(const dcn_paged_cache *cache, const dcn_token_att
     LaunchDevice dev;
     if ((st = launch_device(&dev)) != DCN_OK) return st;
     AttentionParams p{*cache, *args, *q, *out};
+    if (token_attention_tensor(*cache, *args) && packs(*q) && packs(*out))
+        return status_from_cuda(launch_token_attention_tensor(p, workspace, dev.sm_count, dev.err_word,
+                                                              reinterpret_cast<cudaStream_t>(stream)));
     return status_from_cuda(launch_token_attention_direct(p, reinterpret_cast<cudaStream_t>(stream)));
 }
 

@@ -1,0 +1,901 @@
+// dcn_token_attention_sm100.cu -- attention over a paged cache on the tensor cores (FP16, BF16;
+// head_dim 64 and 128).
+//
+// For a row i of queries, over its visible keys s, in one pass with a running maximum m and sum l:
+//   S = Q K^T            tcgen05.mma, Q and K tiles in shared memory, S in tensor memory
+//   P = exp2(c S - c m)  c = scale log2 e; a thread owns a row, so maximum and sum need no exchange
+//   O += P V             tcgen05.mma, P (rounded to the element type) in tensor memory over S
+//   out = O / l
+//
+// A tile is 128 rows by 128 keys.  A key head's q_heads / heads query heads read the same keys, so
+// a tile's rows are (token, query head of that key head): 128 / ratio tokens.  A block runs two
+// streams of tiles, each with its softmax warpgroup and its thread that issues products, so that one
+// stream's exponentials run under the other's products:
+//   shared: two row tiles against the same key tiles (steps of more than 128 rows);
+//   split:  one row tile, each stream with its own range of key tiles (a few tokens).
+// Keys are split further over blocks where rows alone do not fill the GPU; a second, dependent
+// launch joins the parts.
+//
+// Rounding P to the element type (as its values are the second product's operand) costs a relative
+// 2^-12 (FP16) or 2^-9 (BF16) per weight, of the size of the result's own rounding; l sums the
+// unrounded weights in FP32.  The maximum that P is taken against may lag the true one by up to
+// 2^8 before O is rescaled: exact up to the range of P (256 of FP16's 65504), and it spares almost
+// every rescaling.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "dcn_token_attention.cuh"
+#include "dcn_tokens.cuh"
+
+namespace dcn {
+namespace {
+
+constexpr int kRows = 128;          // rows of a tile
+constexpr int kKeys = 128;          // keys of a tile
+constexpr int kSoftmaxWarps = 8;    // two warpgroups
+constexpr int kThreads = 384;       // 2 softmax warpgroups, then 2 product warps, 2 load warps
+constexpr int kTmemCols = 512;      // S0, S1 (128 each), O0, O1 (head_dim each)
+constexpr uint32_t kTmemO = 256;
+constexpr float kLag = 8.0f;        // log2 of how far the maximum in use may lag
+constexpr int kSmCount = 148;
+
+template <int D, bool Shared>
+struct Layout {
+    static constexpr int kRings = Shared ? 1 : 2;
+    static constexpr int kSlots = (Shared ? 5 : 3) * (D == 64 ? 2 : 1);  // tiles of a ring
+    static constexpr int kTileBytes = kKeys * D * 2;
+    static constexpr int kQTiles = Shared ? 2 : 1;
+};
+
+template <int D, bool Shared>
+struct alignas(1024) Smem {
+    using L = Layout<D, Shared>;
+    uint8_t q[L::kQTiles][L::kTileBytes];
+    uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
+    uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
+    uint64_t q_full[2], q_free, s_full[2], p_full[2], o_full[2], scanned[2], drain[2];
+    int dirty[2][2];
+    int abort_flag;
+    uint32_t tmem_base;
+};
+
+struct KernelParams {
+    AttentionParams a;
+    float *part_o;       // [parts][tokens][q_heads][head_dim] unnormalised O; null: write the result
+    float2 *part_ml;     // [parts][tokens][q_heads] (c m, l)
+    uint32_t *err;
+    int ratio;           // query heads of a key head
+    int tile_tokens;     // tokens of a row tile
+    int row_blocks;      // row blocks of the longest step
+    int splits;          // blocks that share one row block's keys
+    int box_rows;        // keys of one TMA box
+    int64_t items;
+    float c;             // |scale| log2 e
+    int negate;          // scale < 0: scores change sign
+};
+
+// The keys that rows at positions p0 .. p1 (0 <= p0 <= p1) see: some row sees [0, pinned) and
+// [low, high), cut to below high; every row sees [0, pinned) and [low_all, high_all), below high_all.
+struct Span {
+    int pinned, low, high, low_all, high_all;
+
+    __device__ __forceinline__ void set(int p0, int p1, int length, const dcn_token_attention_args &a) {
+        const int64_t f0 = p0 / a.frame, f1 = p1 / a.frame;
+        const int64_t high0 = (f0 + 1) * a.frame, high1 = (f1 + 1) * a.frame;
+        const int64_t low0 = (f0 - a.window + 1) * a.frame, low1 = (f1 - a.window + 1) * a.frame;
+        high = static_cast<int>(min(high1, static_cast<int64_t>(length)));
+        high_all = static_cast<int>(min(high0, static_cast<int64_t>(length)));
+        low = static_cast<int>(max(low0, int64_t{0}));
+        low_all = static_cast<int>(max(low1, int64_t{0}));
+        pinned = static_cast<int>(min(static_cast<int64_t>(a.sinks) * a.frame, static_cast<int64_t>(length)));
+    }
+    __device__ __forceinline__ bool some(int key) const { return key < high && (key >= low || key < pinned); }
+    __device__ __forceinline__ bool all(int key) const { return key < high_all && (key >= low_all || key < pinned); }
+    __device__ __forceinline__ bool tile_some(int base) const {
+        return base < high && (base + kKeys > low || base < pinned);
+    }
+    __device__ __forceinline__ bool tile_all(int base) const {
+        return base + kKeys <= high_all && (base >= low_all || base + kKeys <= pinned);
+    }
+};
+
+// One block's work: the rows of up to two tiles against a range of key tiles.  Every role walks the
+// same sequence of items by itself.
+struct Item {
+    int stream, kv_head, start, steps, length;  // steps: the stream's tokens of this step
+    int token0[2], token1[2];  // rows' tokens in the step, per stream of tiles
+    int first[2], last[2];     // range of the list of key tiles, per stream of tiles
+    int pinned_tiles, window_tile;
+    int part[2];
+    Span both;
+
+    __device__ __forceinline__ int key_tile(int i) const {
+        return i < pinned_tiles ? i : window_tile + (i - pinned_tiles);
+    }
+    // First row position with keys of stream of tiles s, and its last.
+    __device__ __forceinline__ int position(int token) const { return length - steps + token; }
+    __device__ __forceinline__ bool has_keys(int s) const {
+        return token1[s] > token0[s] && length > 0 && position(token1[s] - 1) >= 0;
+    }
+    __device__ __forceinline__ void span(int s, const dcn_token_attention_args &a, Span *out) const {
+        out->set(max(position(token0[s]), 0), position(token1[s] - 1), length, a);
+    }
+};
+
+template <bool Shared>
+struct Walk {
+    int64_t w;
+    int block;  // row block, or -1: take the next w
+
+    __device__ __forceinline__ void begin() {
+        w = blockIdx.x;
+        block = -1;
+    }
+    __device__ __forceinline__ bool next(const KernelParams &p, Item &it) {
+        const int block_tokens = p.tile_tokens * (Shared ? 2 : 1);
+        while (w < p.items) {
+            int64_t rest = w;
+            const int split = static_cast<int>(rest % p.splits);
+            rest /= p.splits;
+            // Later row blocks first: under a causal mask they have the most keys.
+            const int first_block = p.row_blocks - 1 - static_cast<int>(rest % p.row_blocks);
+            rest /= p.row_blocks;
+            it.kv_head = static_cast<int>(rest % p.a.cache.heads);
+            it.stream = static_cast<int>(rest / p.a.cache.heads);
+            it.start = p.a.cache.starts[it.stream];
+            it.steps = p.a.cache.starts[it.stream + 1] - it.start;
+            it.length = p.a.cache.lengths[it.stream];
+            // No row outside the token tensors, whatever `starts` holds.
+            const int64_t end_token = min(static_cast<int64_t>(it.steps), p.a.args.tokens - it.start);
+            const int rows_end = it.start < 0 || end_token < 0 ? 0 : static_cast<int>(end_token);
+            // Steps longer than max_q said: every row_blocks-th block is this item's too.
+            block = block < 0 ? first_block : block + p.row_blocks;
+            if (static_cast<int64_t>(block) * block_tokens >= rows_end) {
+                block = -1;
+                w += gridDim.x;
+                continue;
+            }
+            const int t0 = block * block_tokens;
+            it.token0[0] = t0;
+            it.token1[0] = min(t0 + p.tile_tokens, rows_end);
+            it.token0[1] = Shared ? t0 + p.tile_tokens : t0;
+            it.token1[1] = Shared ? min(t0 + 2 * p.tile_tokens, rows_end) : it.token1[0];
+            const int end = max(it.token1[0], it.token1[1]);
+            int tiles = 0;
+            it.pinned_tiles = it.window_tile = 0;
+            if (it.length > 0 && it.position(end - 1) >= 0) {
+                it.both.set(max(it.position(t0), 0), it.position(end - 1), it.length, p.a.args);
+                it.pinned_tiles = (min(it.both.pinned, it.both.high) + kKeys - 1) / kKeys;
+                it.window_tile = max(it.both.low / kKeys, it.pinned_tiles);
+                tiles = it.pinned_tiles + max(0, (it.both.high + kKeys - 1) / kKeys - it.window_tile);
+            }
+            const int parts = Shared ? p.splits : 2 * p.splits;
+            const int each = (tiles + parts - 1) / parts;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                it.part[s] = Shared ? split : 2 * split + s;
+                it.first[s] = min(it.part[s] * each, tiles);
+                it.last[s] = min(it.first[s] + each, tiles);
+            }
+            return true;
+        }
+        return false;
+    }
+};
+
+// Position in a ring of tiles: the slot, and the parity of its current use.
+template <int Slots>
+struct RingAt {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void advance() {
+        if (++slot == Slots) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ bool pair_not_finite(uint32_t w) {
+    constexpr uint32_t kExponent = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+    return (w & kExponent) == kExponent || ((w >> 16) & kExponent) == kExponent;
+}
+
+// One of the failure path's records: some wait ran out.
+template <typename S>
+__device__ __forceinline__ void give_up(S &s, uint32_t *err) {
+    if (*reinterpret_cast<volatile int *>(&s.abort_flag) == 0) atomicOr(err, kErrWaitTimeout);
+    *reinterpret_cast<volatile int *>(&s.abort_flag) = 1;
+}
+
+// out of one row, alone, from its visible keys in key tiles [first, last) of the item's list: for
+// rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in the
+// product would reach the others).  Slow and rare.
+template <typename T, int D>
+__device__ __noinline__ void row_alone(const KernelParams &p, const Item &it, int first, int last, int token, int head,
+                                       const Visible seen, T *out, float *part_o, float2 *part_ml) {
+    const dcn_paged_cache &c = p.a.cache;
+    const T *q = static_cast<const T *>(p.a.q.data) + (it.start + token) * p.a.q.token_stride + head * p.a.q.head_stride;
+    const float sign = p.negate ? -1.0f : 1.0f;
+    float m = -INFINITY, l = 0.0f;
+    for (int e0 = -32; e0 < D; e0 += 32) {  // first the maximum and sum, then 32 elements a pass
+        float acc[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
+        for (int i = first; i < last; ++i) {
+            for (int key = it.key_tile(i) * kKeys; key < (it.key_tile(i) + 1) * kKeys; ++key) {
+                if (!(key < seen.first || (key >= seen.low && key < seen.high))) continue;
+                const int column = key / c.page_size;
+                const int page = column < c.table_columns ? c.table[it.stream * c.table_stride + column] : -1;
+                const bool has = page >= 0 && page < c.pages;
+                const int64_t slot = key - column * c.page_size;
+                float score = 0.0f;
+                if (has) {
+                    const T *k = static_cast<const T *>(c.keys) + page * c.key_page_stride + slot * c.key_slot_stride +
+                                 it.kv_head * c.key_head_stride;
+#pragma unroll 4
+                    for (int e = 0; e < D; e += 8) {
+                        float qv[8], kv[8];
+                        unpack<T, 8>(load_pack<T, 8>(q + e), qv);
+                        unpack<T, 8>(load_pack<T, 8>(k + e), kv);
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) score = fmaf(qv[n] * sign, kv[n], score);
+                    }
+                }
+                score *= p.c;
+                if (e0 < 0) {
+                    const float top = fmaxf(m, score);
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    l = l * exp2_approx(m - base) + exp2_approx(score - base);
+                    m = top;
+                } else if (has) {
+                    const T *v = static_cast<const T *>(c.values) + page * c.value_page_stride +
+                                 slot * c.value_slot_stride + it.kv_head * c.value_head_stride + e0;
+                    const float w = exp2_approx(score - (m == -INFINITY ? 0.0f : m));
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float vv[8];
+                        unpack<T, 8>(load_pack<T, 8>(v + e), vv);
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) acc[e + n] = fmaf(w, vv[n], acc[e + n]);
+                    }
+                }
+            }
+        }
+        if (e0 < 0) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            if (part_o) part_o[e0 + e] = acc[e];
+            else out[e0 + e] = from_float<T>(seen.first <= 0 && seen.high <= seen.low ? 0.0f : acc[e] / l);
+        }
+    }
+    if (part_o) *part_ml = make_float2(m, l);
+}
+
+template <typename T, int D, bool Shared>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__ CUtensorMap k_map,
+                 const __grid_constant__ CUtensorMap v_map) {
+    using L = Layout<D, Shared>;
+    extern __shared__ uint8_t raw[];
+    Smem<D, Shared> &sm = *reinterpret_cast<Smem<D, Shared> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
+    volatile int *abort_flag = &sm.abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int r = 0; r < L::kRings; ++r)
+            for (int i = 0; i < L::kSlots; ++i) {
+                mbar_init(&sm.full[r][i], 1);
+                mbar_init(&sm.empty[r][i], Shared ? 2 : 1);
+            }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sm.q_full[s], kRows);
+            mbar_init(&sm.s_full[s], 1);
+            mbar_init(&sm.p_full[s], 4);
+            mbar_init(&sm.o_full[s], 1);
+            mbar_init(&sm.scanned[s], 4);
+            mbar_init(&sm.drain[s], 1);
+            sm.dirty[s][0] = sm.dirty[s][1] = -1;
+        }
+        mbar_init(&sm.q_free, 1);
+        sm.abort_flag = 0;
+        fence_mbarrier_init();
+        prefetch_tensor_map(&k_map);
+        prefetch_tensor_map(&v_map);
+    }
+    if (warp == kSoftmaxWarps) {
+        tmem_alloc(&sm.tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    if (p.part_o) allow_dependent_launch();
+
+    if (warp >= kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int s = (warp - kSoftmaxWarps) & 1;
+        if (warp < kSoftmaxWarps + 2) {
+            if (lane == 0) {
+                // ------------------------------------------------------------ products of stream s
+                constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+                constexpr uint32_t kTypes = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+                constexpr uint32_t kIdescS = make_idesc_f16_f32(kRows, kKeys) | kTypes;
+                constexpr uint32_t kIdescO = make_idesc_f16_f32(kRows, D) | kTypes | (1u << 16);  // B: N contiguous
+                const int ring = Shared ? 0 : s;
+                const uint32_t s_tmem = tmem + s * kKeys, o_tmem = tmem + kTmemO + s * D;
+                const uint32_t q_base = smem_addr(sm.q[Shared ? s : 0]);
+                RingAt<L::kSlots> at;
+                uint32_t q_phase = 0, p_phase = 0;
+                bool ok = true;
+                auto wait = [&](uint64_t *bar, uint32_t parity) {
+                    if (ok && !mbar_wait_bounded(bar, parity, abort_flag)) {
+                        give_up(sm, p.err);
+                        ok = false;
+                    }
+                    return ok;
+                };
+                Walk<Shared> walk;
+                Item it;
+                for (walk.begin(); ok && walk.next(p, it);) {
+                    Span span;
+                    const bool rows = it.token1[s] > it.token0[s];
+                    const bool keys = it.has_keys(s);
+                    if (keys) it.span(s, p.a.args, &span);
+                    if (rows) {
+                        if (!wait(&sm.q_full[Shared ? s : 0], q_phase)) break;
+                        q_phase ^= 1u;
+                    }
+                    uint32_t more = 0;
+                    for (int i = it.first[s]; ok && i < it.last[s]; ++i) {
+                        const bool take = keys && span.tile_some(it.key_tile(i) * kKeys);
+                        if (!wait(&sm.full[ring][at.slot], at.parity)) break;
+                        if (take) {
+                            tc_fence_after();
+                            const uint32_t k_base = smem_addr(sm.kv[ring][at.slot]);
+#pragma unroll
+                            for (int d = 0; d < D; d += 16) {
+                                const uint32_t off = (d / 64) * (kKeys * 128) + (d % 64) * 2;
+                                umma_f16_ss(s_tmem, make_sw128_kmajor_desc(q_base + off),
+                                            make_sw128_kmajor_desc(k_base + off), kIdescS, d != 0);
+                            }
+                            umma_commit(&sm.s_full[s]);
+                            umma_commit(&sm.empty[ring][at.slot]);
+                        } else {
+                            mbar_arrive(&sm.empty[ring][at.slot]);
+                        }
+                        at.advance();
+                        if (!wait(&sm.full[ring][at.slot], at.parity)) break;
+                        if (take) {
+                            if (!wait(&sm.p_full[s], p_phase)) break;
+                            p_phase ^= 1u;
+                            tc_fence_after();
+                            const uint32_t v_base = smem_addr(sm.kv[ring][at.slot]);
+#pragma unroll
+                            for (int k = 0; k < kKeys; k += 16) {
+                                umma_f16_ts(o_tmem, s_tmem + k / 2, make_sw128_mnmajor_desc(v_base + k * 128, kKeys * 128),
+                                            kIdescO, more);
+                                more = 1;
+                            }
+                            umma_commit(&sm.empty[ring][at.slot]);
+                        } else {
+                            mbar_arrive(&sm.empty[ring][at.slot]);
+                        }
+                        at.advance();
+                    }
+                    // Once an item, with or without products: the softmax warpgroup moves on only after it,
+                    // so no barrier of the item runs a phase ahead of this thread.
+                    if (ok && rows) {
+                        umma_commit(&sm.o_full[s]);
+                        if (!Shared && s == 1) umma_commit(&sm.q_free);
+                    }
+                }
+                // Every product issued has ended before the block lets go of its memory.
+                umma_commit(&sm.drain[s]);
+                mbar_wait_bounded(&sm.drain[s], 0, nullptr);
+            }
+        } else if (s < L::kRings) {
+            // -------------------------------------------------------------------- loads of ring s
+            RingAt<L::kSlots> at;
+            uint32_t loaded = 0;
+            const int groups = kKeys / p.box_rows, boxes = groups * (D / 64);
+            bool ok = true;
+            Walk<Shared> walk;
+            Item it;
+            for (walk.begin(); ok && walk.next(p, it);) {
+                for (int i = it.first[s]; ok && i < it.last[s]; ++i) {
+                    // Box b of a tile: keys [group * box_rows, ...) and 64 elements.
+                    const int group = lane % groups, half = lane / groups;
+                    const int key = it.key_tile(i) * kKeys + group * p.box_rows;
+                    const int column = key / p.a.cache.page_size;
+                    int page = -1;  // outside the cache: the copy fills with zeros
+                    if (lane < boxes && key < it.length && column < p.a.cache.table_columns) {
+                        page = p.a.cache.table[it.stream * p.a.cache.table_stride + column];
+                        if (page < 0 || page >= p.a.cache.pages) page = -1;
+                    }
+                    const int slot = key - column * p.a.cache.page_size;
+#pragma unroll 1
+                    for (int v = 0; v < 2; ++v) {
+                        ok = mbar_wait_bounded(&sm.empty[s][at.slot], at.parity ^ 1u, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            if (lane == 0) give_up(sm, p.err);
+                            break;
+                        }
+                        if (lane == 0) mbar_arrive_expect_tx(&sm.full[s][at.slot], L::kTileBytes);
+                        __syncwarp();
+                        if (lane < boxes)
+                            tma_load_4d(sm.kv[s][at.slot] + half * (kKeys * 128) + group * p.box_rows * 128,
+                                        v == 0 ? &k_map : &v_map, &sm.full[s][at.slot], half * 64, slot, it.kv_head, page);
+                        at.advance();
+                        ++loaded;
+                    }
+                }
+            }
+            // Every copy issued has landed before the block lets go of its memory.
+            for (uint32_t k = 0; k < L::kSlots && k < loaded; ++k) {
+                const uint32_t last = loaded - 1 - k;
+                mbar_wait_bounded(&sm.full[s][last % L::kSlots], (last / L::kSlots) & 1u, nullptr);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---------------------------------------------------------------------- softmax of stream s
+        const int s = warp >> 2;
+        const int row = threadIdx.x & (kRows - 1);
+        const int ring = Shared ? 0 : s;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_tmem = tmem + lanes + s * kKeys, o_tmem = tmem + lanes + kTmemO + s * D;
+        const int row_token = row / p.ratio, row_head = row - row_token * p.ratio;
+        const bool row_used = row_token < p.tile_tokens;
+        RingAt<L::kSlots> at;
+        uint32_t s_phase = 0, item_phase = 0, free_phase = 0;
+        int item_number = 0;
+        bool ok = true, q_loaded = false;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {  // the whole warp gives up together
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+            if (!ok && lane == 0) give_up(sm, p.err);
+            return ok;
+        };
+        Walk<Shared> walk;
+        Item it;
+        for (walk.begin(); ok && walk.next(p, it); ++item_number) {
+            const bool rows = it.token1[s] > it.token0[s];
+            const bool keys = it.has_keys(s);
+            const int token = it.token0[s] + row_token;
+            const int head = it.kv_head * p.ratio + row_head;
+            const bool valid = row_used && token < it.token1[s];
+            if (rows && (Shared || s == 0)) {
+                if (!Shared && q_loaded) {  // the other stream's products have read the last tile
+                    if (!wait(&sm.q_free, free_phase)) break;
+                    free_phase ^= 1u;
+                }
+                q_loaded = true;
+                // 16 bytes a load, a row's packs on neighbouring threads.
+                constexpr int kPacks = D / 8;
+                const T *q = static_cast<const T *>(p.a.q.data);
+                uint4 v[kPacks];
+#pragma unroll
+                for (int i = 0; i < kPacks; ++i) {
+                    const int r = (i * kRows + row) / kPacks, e = (row % kPacks) * 8;
+                    const int rt = r / p.ratio, rh = r - rt * p.ratio;
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (rt < p.tile_tokens && it.token0[s] + rt < it.token1[s])
+                        v[i] = *reinterpret_cast<const uint4 *>(q + (it.start + it.token0[s] + rt) * p.a.q.token_stride +
+                                                                (it.kv_head * p.ratio + rh) * p.a.q.head_stride + e);
+                }
+#pragma unroll
+                for (int i = 0; i < kPacks; ++i) {
+                    const int r = (i * kRows + row) / kPacks, e = row % kPacks;
+                    if (p.negate) {
+                        v[i].x ^= 0x80008000u;
+                        v[i].y ^= 0x80008000u;
+                        v[i].z ^= 0x80008000u;
+                        v[i].w ^= 0x80008000u;
+                    }
+                    // 128-byte swizzle: pack e of a row goes to place e ^ (row mod 8) of its 8.
+                    uint8_t *dst = sm.q[Shared ? s : 0] + (e / 8) * (kRows * 128) + r * 128 + (((e % 8) ^ (r % 8)) * 16);
+                    *reinterpret_cast<uint4 *>(dst) = v[i];
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&sm.q_full[s]);
+            }
+            Span span;
+            if (keys) it.span(s, p.a.args, &span);
+            const Visible seen = visible_keys(it.position(token), it.length, p.a.args.window, p.a.args.sinks, p.a.args.frame);
+            const int seen_first = static_cast<int>(seen.first), seen_low = static_cast<int>(seen.low),
+                      seen_high = static_cast<int>(seen.high);
+            const bool warp_used = __any_sync(0xffffffffu, valid);
+            float m = -INFINITY, l = 0.0f;
+            bool any = false;
+            for (int i = it.first[s]; i < it.last[s]; ++i) {
+                const int base = it.key_tile(i) * kKeys;
+                if (!(keys && span.tile_some(base))) {
+                    at.advance();
+                    at.advance();
+                    continue;
+                }
+                at.advance();  // the values' slot
+                if (!span.tile_all(base)) {
+                    // Some rows' weights are 0 for some keys here, and 0 x non-finite is not 0.  A key that
+                    // no row of the block sees becomes zeros; where only some see it, all rows are done alone.
+                    if (!wait(&sm.full[ring][at.slot], at.parity)) break;
+                    const int key = base + row;
+                    if (!span.all(key)) {
+                        uint8_t *v_row = sm.kv[ring][at.slot] + row * 128;
+                        const bool hidden = !it.both.some(key);
+#pragma unroll
+                        for (int e = 0; e < D / 8; ++e) {
+                            uint4 *at16 = reinterpret_cast<uint4 *>(v_row + (e / 8) * (kKeys * 128) + (((e % 8) ^ (row % 8)) * 16));
+                            const uint4 v = *at16;
+                            if (pair_not_finite<T>(v.x) || pair_not_finite<T>(v.y) || pair_not_finite<T>(v.z) ||
+                                pair_not_finite<T>(v.w)) {
+                                if (hidden) *at16 = make_uint4(0, 0, 0, 0);
+                                else *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) = item_number;
+                            }
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                at.advance();
+                if (!wait(&sm.s_full[s], s_phase)) break;
+                s_phase ^= 1u;
+                if (warp_used) {
+                    tc_fence_after();
+                    uint32_t x[kKeys];
+#pragma unroll
+                    for (int k = 0; k < kKeys; k += 32) tmem_ld_32x32b_x32(s_tmem + k, x + k);
+#pragma unroll
+                    for (int k = 0; k < kKeys; k += 32) tmem_wait_ld_x32(x + k);
+                    const bool clear = !valid || base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high);
+                    if (!__all_sync(0xffffffffu, clear)) {
+                        if (!clear) {
+                            const int a = seen_first - base, lo = seen_low - base, hi = seen_high - base;
+#pragma unroll
+                            for (int k = 0; k < kKeys; ++k)
+                                if (!(k < a || (k >= lo && k < hi))) x[k] = 0xff800000u;  // -inf
+                        }
+                        __syncwarp();
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = __uint_as_float(x[j]);
+#pragma unroll
+                    for (int k = 4; k < kKeys; k += 4)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[k + j]));
+                    const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    if (!any) {
+                        m = t;
+                    } else if (__any_sync(0xffffffffu, (t - m) * p.c > kLag)) {
+                        // Products up to the last tile's have ended: S of this tile was issued after them.
+                        const float to = fmaxf(m, t);
+                        const float shrink = to == -INFINITY ? 1.0f : exp2_approx((m - to) * p.c);
+                        m = to;
+                        l *= shrink;
+#pragma unroll
+                        for (int d = 0; d < D; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(o_tmem + d, o);
+                            tmem_wait_ld_x32(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                            tmem_st_32x32b_x32_wait(o_tmem + d, o);
+                        }
+                    }
+                    const float mc = m == -INFINITY ? 0.0f : m * p.c;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < kKeys; k += 2) {
+                        const float a = exp2_approx(fmaf(__uint_as_float(x[k]), p.c, -mc));
+                        const float b = exp2_approx(fmaf(__uint_as_float(x[k + 1]), p.c, -mc));
+                        sum[k / 2 % 4] += a + b;
+                        x[k / 2] = pack_pair<T>(a, b);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st_32x32b_x32_wait(s_tmem, x);
+                    tmem_st_32x32b_x32_wait(s_tmem + 32, x + 32);
+                    tc_fence_before();
+                    __syncwarp();
+                }
+                any = true;
+                if (lane == 0) mbar_arrive(&sm.p_full[s]);
+            }
+            if (!ok) break;
+            if (!rows) continue;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.scanned[s]);
+            if (!wait(&sm.o_full[s], item_phase) || !wait(&sm.scanned[s], item_phase)) break;
+            item_phase ^= 1u;
+            tc_fence_after();
+            const bool alone = *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) == item_number;
+            const int64_t at_row = static_cast<int64_t>(it.start + token) * p.a.args.q_heads + head;
+            const int64_t part_row = static_cast<int64_t>(it.part[s]) * p.a.args.tokens * p.a.args.q_heads + at_row;
+            T *out = static_cast<T *>(p.a.out.data) + (it.start + token) * p.a.out.token_stride + head * p.a.out.head_stride;
+            if (alone) {
+                if (valid)
+                    row_alone<T, D>(p, it, it.first[s], it.last[s], token, head, seen, out,
+                                    p.part_o ? p.part_o + part_row * D : nullptr, p.part_ml ? p.part_ml + part_row : nullptr);
+                continue;
+            }
+            if (!warp_used) continue;
+            const bool none = seen_first <= 0 && seen_high <= seen_low;
+            if (p.part_o) {
+                if (valid) p.part_ml[part_row] = any ? make_float2(m * p.c, l) : make_float2(-INFINITY, 0.0f);
+                if (!any) continue;  // a part without weight is not read
+            }
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                if (any) {
+                    tmem_ld_32x32b_x32(o_tmem + d, o);
+                    tmem_wait_ld_x32(o);
+                }
+                if (valid && p.part_o) {
+                    float4 *dst = reinterpret_cast<float4 *>(p.part_o + part_row * D + d);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                             __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+                } else if (valid) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(out + d);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            w[n] = none ? 0u : pack_pair<T>(__uint_as_float(o[8 * j + 2 * n]) * inv,
+                                                            __uint_as_float(o[8 * j + 2 * n + 1]) * inv);
+                        dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kSoftmaxWarps) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the parts of a row: out = sum_j 2^(M_j - M) O_j / sum_j 2^(M_j - M) l_j, M the largest of
+// the parts' maxima M_j (in log2).  One warp a row; parts in their order, so the result does not
+// depend on which block was first.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ KernelParams p, int parts) {
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int64_t rows = p.a.args.tokens * p.a.args.q_heads;
+    const int64_t token = row / p.a.args.q_heads;
+    const int head = static_cast<int>(row - token * p.a.args.q_heads);
+    const int b = row < rows ? find_stream(p.a.cache.starts, p.a.cache.streams, token) : p.a.cache.streams;
+    grid_dependency_wait();
+    if (b >= p.a.cache.streams) return;  // padding past the last stream
+    const int64_t length = p.a.cache.lengths[b];
+    const Visible seen = visible_keys(length - p.a.cache.starts[b + 1] + token, length, p.a.args.window, p.a.args.sinks,
+                                      p.a.args.frame);
+    float top = -INFINITY;
+    for (int j = lane; j < parts; j += 32) top = fmaxf(top, p.part_ml[j * rows + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    constexpr int kPer = D / 32;
+    float acc[kPer], sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+    for (int j = 0; j < parts; ++j) {
+        const float2 ml = p.part_ml[j * rows + row];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing visible in this part
+        const float w = exp2_approx(ml.x - base);
+        sum = fmaf(w, ml.y, sum);
+        const float *o = p.part_o + (j * rows + row) * D + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(w, o[e], acc[e]);
+    }
+    const bool none = seen.first <= 0 && seen.high <= seen.low;
+    T *out = static_cast<T *>(p.a.out.data) + token * p.a.out.token_stride + head * p.a.out.head_stride + lane * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) out[e] = from_float<T>(none ? 0.0f : acc[e] / sum);
+}
+
+// ---- host side -------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// Keys of one TMA box: the largest power of two that divides the page, at most a tile.
+int box_rows(int page_size) {
+    int rows = 8;
+    while (rows < kKeys && page_size % (rows * 2) == 0) rows *= 2;
+    return rows;
+}
+
+bool page_map(CUtensorMap *map, const dcn_paged_cache &c, void *base, int64_t slot, int64_t head, int64_t page) {
+    auto fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(slot) * 2, static_cast<cuuint64_t>(head) * 2,
+                                   static_cast<cuuint64_t>(page) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows(c.page_size)), 1, 1};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    return fn(map, c.dtype == DCN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base,
+              dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+    bool shared;
+    int ratio, tile_tokens, row_blocks, splits, parts;  // parts == 0: no join
+    int64_t items;
+};
+
+Plan make_plan(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
+    Plan plan{};
+    plan.ratio = a.q_heads / c.heads;
+    plan.tile_tokens = kRows / plan.ratio;
+    plan.shared = a.max_q > plan.tile_tokens;
+    const int block_tokens = plan.tile_tokens * (plan.shared ? 2 : 1);
+    plan.row_blocks = a.max_q > 0 ? (a.max_q - 1) / block_tokens + 1 : 1;
+    const int64_t blocks = static_cast<int64_t>(plan.row_blocks) * c.heads * c.streams;
+    // Key tiles of a row block, at most.
+    auto keys_of = [&](int32_t frames) {
+        return frames > a.max_kv / a.frame ? int64_t{a.max_kv} : static_cast<int64_t>(frames) * a.frame;
+    };
+    const int64_t span = keys_of(a.window) + keys_of(a.sinks) + block_tokens;
+    const int64_t tiles = (span < a.max_kv ? span : a.max_kv) / kKeys + 1;
+    // Split the keys of a row block over as many blocks as make the whole shortest: rounds of the
+    // GPU's blocks, each as long as its tiles plus a fixed part (start, queries, result), plus the join.
+    const int streams = plan.shared ? 1 : 2;
+    int64_t best = INT64_MAX;
+    plan.splits = 1;
+    for (int s = 1; s <= 64 && (s == 1 || s * streams <= tiles); ++s) {
+        const int64_t rounds = (blocks * s + kSmCount - 1) / kSmCount;
+        const int64_t cost = rounds * ((tiles + s * streams - 1) / (s * streams) + 3) + (plan.shared && s > 1 ? 6 : 0);
+        if (cost < best) {
+            best = cost;
+            plan.splits = s;
+        }
+    }
+    plan.parts = plan.shared && plan.splits == 1 ? 0 : plan.splits * streams;
+    plan.items = blocks * plan.splits;
+    return plan;
+}
+
+int64_t part_rows(const Plan &plan, const dcn_token_attention_args &a) {
+    return static_cast<int64_t>(plan.parts) * a.tokens * a.q_heads;
+}
+
+template <typename T, int D, bool Shared>
+cudaError_t launch(const KernelParams &k, const Plan &plan, const CUtensorMap &k_map, const CUtensorMap &v_map, int sm_count,
+                   cudaStream_t stream) {
+    const int grid = static_cast<int>(k.items < sm_count ? k.items : sm_count);
+    attention_kernel<T, D, Shared><<<grid, kThreads, sizeof(Smem<D, Shared>) + 1024, stream>>>(k, k_map, v_map);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || plan.parts == 0) return e;
+    const int64_t rows = k.a.args.tokens * k.a.args.q_heads;
+    return launch_dependent(attention_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream, k,
+                            plan.parts);
+}
+
+template <typename T>
+cudaError_t launch_typed(const KernelParams &k, const Plan &plan, const CUtensorMap &k_map, const CUtensorMap &v_map,
+                         int sm_count, cudaStream_t stream) {
+    if (k.a.cache.head_dim == 64)
+        return plan.shared ? launch<T, 64, true>(k, plan, k_map, v_map, sm_count, stream)
+                           : launch<T, 64, false>(k, plan, k_map, v_map, sm_count, stream);
+    return plan.shared ? launch<T, 128, true>(k, plan, k_map, v_map, sm_count, stream)
+                       : launch<T, 128, false>(k, plan, k_map, v_map, sm_count, stream);
+}
+
+template <typename T, int D, bool Shared>
+cudaError_t prepare() {
+    const void *fn = reinterpret_cast<const void *>(attention_kernel<T, D, Shared>);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(sizeof(Smem<D, Shared>) + 1024));
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, fn);
+    if (e != cudaSuccess) return e;
+    // The softmax warps grow to 224 registers out of what the block starts with (8 x 224 + 4 x 56 = 12 x 168).
+    if (attr.maxThreadsPerBlock < kThreads || attr.numRegs < 168) return cudaErrorInvalidConfiguration;
+    return cudaSuccess;
+}
+
+}  // namespace
+
+bool token_attention_tensor(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
+    if (c.dtype != DCN_DTYPE_F16 && c.dtype != DCN_DTYPE_BF16) return false;
+    if ((c.head_dim != 64 && c.head_dim != 128) || a.q_heads / c.heads > kRows || c.page_size % 8 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(c.keys) % 16 != 0 || reinterpret_cast<uintptr_t>(c.values) % 16 != 0) return false;
+    const int64_t strides[] = {c.key_page_stride,   c.key_slot_stride,   c.key_head_stride,
+                               c.value_page_stride, c.value_slot_stride, c.value_head_stride};
+    for (int64_t s : strides)
+        if (s <= 0 || s % 8 != 0 || s >= (int64_t{1} << 39)) return false;
+    return true;
+}
+
+size_t token_attention_tensor_workspace(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
+    const int64_t rows = part_rows(make_plan(c, a), a);
+    return static_cast<size_t>(rows) * (c.head_dim * sizeof(float) + sizeof(float2));
+}
+
+cudaError_t token_attention_prepare_device() {
+    cudaError_t e = prepare<__half, 64, true>();
+    if (e == cudaSuccess) e = prepare<__half, 64, false>();
+    if (e == cudaSuccess) e = prepare<__half, 128, true>();
+    if (e == cudaSuccess) e = prepare<__half, 128, false>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16, 64, true>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16, 64, false>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16, 128, true>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16, 128, false>();
+    return e;
+}
+
+cudaError_t launch_token_attention_tensor(const AttentionParams &a, void *workspace, int sm_count, uint32_t *err,
+                                          cudaStream_t stream) {
+    const Plan plan = make_plan(a.cache, a.args);
+    KernelParams k{};
+    k.a = a;
+    if (plan.parts > 0) {
+        k.part_o = static_cast<float *>(workspace);
+        k.part_ml = reinterpret_cast<float2 *>(k.part_o + part_rows(plan, a.args) * a.cache.head_dim);
+    }
+    k.err = err;
+    k.ratio = plan.ratio;
+    k.tile_tokens = plan.tile_tokens;
+    k.row_blocks = plan.row_blocks;
+    k.splits = plan.splits;
+    k.box_rows = box_rows(a.cache.page_size);
+    k.items = plan.items;
+    // Above zero, so that a hidden key's score of -inf stays -inf; 1e-30 makes every weight 1 as 0 would.
+    const float c = fabsf(a.args.scale) * 1.4426950408889634f;
+    k.c = c > 1e-30f ? c : 1e-30f;
+    k.negate = a.args.scale < 0.0f;
+    CUtensorMap k_map, v_map;
+    const dcn_paged_cache &cache = a.cache;
+    if (!page_map(&k_map, cache, cache.keys, cache.key_slot_stride, cache.key_head_stride, cache.key_page_stride) ||
+        !page_map(&v_map, cache, cache.values, cache.value_slot_stride, cache.value_head_stride, cache.value_page_stride))
+        return cudaErrorInvalidValue;
+    return a.cache.dtype == DCN_DTYPE_F16 ? launch_typed<__half>(k, plan, k_map, v_map, sm_count, stream)
+                                          : launch_typed<__nv_bfloat16>(k, plan, k_map, v_map, sm_count, stream);
+}
+
+}  // namespace dcn

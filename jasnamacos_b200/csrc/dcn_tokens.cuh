@@ -50,6 +50,14 @@ struct AttentionParams {
 
 cudaError_t launch_token_attention_direct(const AttentionParams &p, cudaStream_t stream);
 
+// The tensor-core kernel: whether it takes a cache and arguments, its scratch, its set-up (once per
+// device and context), its launch.
+bool token_attention_tensor(const dcn_paged_cache &c, const dcn_token_attention_args &a);
+size_t token_attention_tensor_workspace(const dcn_paged_cache &c, const dcn_token_attention_args &a);
+cudaError_t token_attention_prepare_device();
+cudaError_t launch_token_attention_tensor(const AttentionParams &p, void *workspace, int sm_count, uint32_t *err,
+                                          cudaStream_t stream);
+
 #if defined(__CUDACC__)
 
 // ---- elements ------------------------------------------------------------------------
