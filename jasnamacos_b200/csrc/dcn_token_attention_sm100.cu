@@ -49,18 +49,6 @@ struct Layout {
     static constexpr int kQTiles = Shared ? 2 : 1;
 };
 
-template <int D, bool Shared>
-struct alignas(1024) Smem {
-    using L = Layout<D, Shared>;
-    uint8_t q[L::kQTiles][L::kTileBytes];
-    uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
-    uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
-    uint64_t q_full[2], q_free, s_full[2], p_full[2], o_full[2], scanned[2], drain[2];
-    int dirty[2][2];
-    int abort_flag;
-    uint32_t tmem_base;
-};
-
 struct KernelParams {
     AttentionParams a;
     float *part_o;       // [parts][tokens][q_heads][head_dim] unnormalised O; null: write the result
@@ -71,7 +59,7 @@ struct KernelParams {
     int row_blocks;      // row blocks of the longest step
     int splits;          // blocks that share one row block's keys
     int box_rows;        // keys of one TMA box
-    int64_t items;
+    int items;
     float c;             // |scale| log2 e
     int negate;          // scale < 0: scores change sign
 };
@@ -101,49 +89,57 @@ struct Span {
     }
 };
 
-// One block's work: the rows of up to two tiles against a range of key tiles.  Every role walks the
-// same sequence of items by itself.
+// One block's work for one of its two streams of tiles: the rows of a tile against a range of key
+// tiles.  Every role walks the same sequence of items by itself.
 struct Item {
     int stream, kv_head, start, steps, length;  // steps: the stream's tokens of this step
-    int token0[2], token1[2];  // rows' tokens in the step, per stream of tiles
-    int first[2], last[2];     // range of the list of key tiles, per stream of tiles
-    int pinned_tiles, window_tile;
-    int part[2];
-    Span both;
+    int token0, token1;             // the tile's tokens in the step
+    int first, last;                // range of the list of key tiles
+    int pinned_tiles, window_tile;  // the list: tiles [0, pinned_tiles), then from window_tile
+    int part;
+    Span both;                      // of the rows of both streams
 
     __device__ __forceinline__ int key_tile(int i) const {
         return i < pinned_tiles ? i : window_tile + (i - pinned_tiles);
     }
-    // First row position with keys of stream of tiles s, and its last.
     __device__ __forceinline__ int position(int token) const { return length - steps + token; }
-    __device__ __forceinline__ bool has_keys(int s) const {
-        return token1[s] > token0[s] && length > 0 && position(token1[s] - 1) >= 0;
+    __device__ __forceinline__ bool rows() const { return token1 > token0; }
+    // Whether some row of the tile has a position in the stream, and what such rows see.
+    __device__ __forceinline__ bool keys() const { return rows() && length > 0 && position(token1 - 1) >= 0; }
+    // Bit j: whether the tile's rows see some key of tile i + j of the block's range (a whole warp's call).
+    __device__ __forceinline__ uint32_t takes(int i, int lane, const dcn_token_attention_args &a) const {
+        const int at = first + i + lane;
+        return __ballot_sync(0xffffffffu, keys() && at < last && span(a).tile_some(key_tile(at) * kKeys));
     }
-    __device__ __forceinline__ void span(int s, const dcn_token_attention_args &a, Span *out) const {
-        out->set(max(position(token0[s]), 0), position(token1[s] - 1), length, a);
+    // Of those, the tiles that some of its rows do not see all of.
+    __device__ __forceinline__ uint32_t cuts(int i, int lane, const dcn_token_attention_args &a) const {
+        const int at = first + i + lane;
+        return __ballot_sync(0xffffffffu, keys() && at < last && !span(a).tile_all(key_tile(at) * kKeys));
+    }
+    __device__ __forceinline__ Span span(const dcn_token_attention_args &a) const {
+        Span out;
+        out.set(max(position(token0), 0), position(token1 - 1), length, a);
+        return out;
     }
 };
 
 template <bool Shared>
 struct Walk {
-    int64_t w;
-    int block;  // row block, or -1: take the next w
+    int w, block;  // item, and its row block (-1: take the item's first)
+    int s;         // stream of tiles
 
-    __device__ __forceinline__ void begin() {
-        w = blockIdx.x;
-        block = -1;
-    }
+    __device__ __forceinline__ explicit Walk(int stream_of_tiles) : w(blockIdx.x), block(-1), s(stream_of_tiles) {}
     __device__ __forceinline__ bool next(const KernelParams &p, Item &it) {
         const int block_tokens = p.tile_tokens * (Shared ? 2 : 1);
         while (w < p.items) {
-            int64_t rest = w;
-            const int split = static_cast<int>(rest % p.splits);
+            int rest = w;
+            const int split = rest % p.splits;
             rest /= p.splits;
             // Later row blocks first: under a causal mask they have the most keys.
-            const int first_block = p.row_blocks - 1 - static_cast<int>(rest % p.row_blocks);
+            const int first_block = p.row_blocks - 1 - rest % p.row_blocks;
             rest /= p.row_blocks;
-            it.kv_head = static_cast<int>(rest % p.a.cache.heads);
-            it.stream = static_cast<int>(rest / p.a.cache.heads);
+            it.kv_head = rest % p.a.cache.heads;
+            it.stream = rest / p.a.cache.heads;
             it.start = p.a.cache.starts[it.stream];
             it.steps = p.a.cache.starts[it.stream + 1] - it.start;
             it.length = p.a.cache.lengths[it.stream];
@@ -157,12 +153,9 @@ struct Walk {
                 w += gridDim.x;
                 continue;
             }
-            const int t0 = block * block_tokens;
-            it.token0[0] = t0;
-            it.token1[0] = min(t0 + p.tile_tokens, rows_end);
-            it.token0[1] = Shared ? t0 + p.tile_tokens : t0;
-            it.token1[1] = Shared ? min(t0 + 2 * p.tile_tokens, rows_end) : it.token1[0];
-            const int end = max(it.token1[0], it.token1[1]);
+            const int t0 = block * block_tokens, end = min(t0 + block_tokens, rows_end);
+            it.token0 = Shared ? t0 + s * p.tile_tokens : t0;
+            it.token1 = min(it.token0 + p.tile_tokens, rows_end);
             int tiles = 0;
             it.pinned_tiles = it.window_tile = 0;
             if (it.length > 0 && it.position(end - 1) >= 0) {
@@ -173,16 +166,27 @@ struct Walk {
             }
             const int parts = Shared ? p.splits : 2 * p.splits;
             const int each = (tiles + parts - 1) / parts;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                it.part[s] = Shared ? split : 2 * split + s;
-                it.first[s] = min(it.part[s] * each, tiles);
-                it.last[s] = min(it.first[s] + each, tiles);
-            }
+            it.part = Shared ? split : 2 * split + s;
+            it.first = min(it.part * each, tiles);
+            it.last = min(it.first + each, tiles);
             return true;
         }
         return false;
     }
+};
+
+template <int D, bool Shared>
+struct alignas(1024) Smem {
+    using L = Layout<D, Shared>;
+    uint8_t q[L::kQTiles][L::kTileBytes];
+    uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
+    uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
+    uint64_t q_full[2], q_free, s_full[2], p_full[2], o_full[2], scanned[2], drain;
+    // Each softmax warp's current item, kept here: the 128 scores of a row need the registers.
+    Item item[kSoftmaxWarps];
+    int dirty[2][2];
+    int abort_flag;
+    uint32_t tmem_base;
 };
 
 // Position in a ring of tiles: the slot, and the parity of its current use.
@@ -234,8 +238,8 @@ __device__ __forceinline__ void give_up(S &s, uint32_t *err) {
 // rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in the
 // product would reach the others).  Slow and rare.
 template <typename T, int D>
-__device__ __noinline__ void row_alone(const KernelParams &p, const Item &it, int first, int last, int token, int head,
-                                       const Visible seen, T *out, float *part_o, float2 *part_ml) {
+__device__ __noinline__ void row_alone(const KernelParams &p, const Item it, int token, int head, const Visible seen, T *out,
+                                       float *part_o, float2 *part_ml) {
     const dcn_paged_cache &c = p.a.cache;
     const T *q = static_cast<const T *>(p.a.q.data) + (it.start + token) * p.a.q.token_stride + head * p.a.q.head_stride;
     const float sign = p.negate ? -1.0f : 1.0f;
@@ -244,7 +248,7 @@ __device__ __noinline__ void row_alone(const KernelParams &p, const Item &it, in
         float acc[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-        for (int i = first; i < last; ++i) {
+        for (int i = it.first; i < it.last; ++i) {
             for (int key = it.key_tile(i) * kKeys; key < (it.key_tile(i) + 1) * kKeys; ++key) {
                 if (!(key < seen.first || (key >= seen.low && key < seen.high))) continue;
                 const int column = key / c.page_size;
@@ -308,7 +312,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         for (int r = 0; r < L::kRings; ++r)
             for (int i = 0; i < L::kSlots; ++i) {
                 mbar_init(&sm.full[r][i], 1);
-                mbar_init(&sm.empty[r][i], Shared ? 2 : 1);
+                mbar_init(&sm.empty[r][i], 1);
             }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.q_full[s], kRows);
@@ -316,10 +320,10 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             mbar_init(&sm.p_full[s], 4);
             mbar_init(&sm.o_full[s], 1);
             mbar_init(&sm.scanned[s], 4);
-            mbar_init(&sm.drain[s], 1);
             sm.dirty[s][0] = sm.dirty[s][1] = -1;
         }
         mbar_init(&sm.q_free, 1);
+        mbar_init(&sm.drain, 1);
         sm.abort_flag = 0;
         fence_mbarrier_init();
         prefetch_tensor_map(&k_map);
@@ -336,97 +340,116 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
     if (p.part_o) allow_dependent_launch();
 
     if (warp >= kSoftmaxWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        const int s = (warp - kSoftmaxWarps) & 1;
-        if (warp < kSoftmaxWarps + 2) {
-            if (lane == 0) {
-                // ------------------------------------------------------------ products of stream s
-                constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
-                constexpr uint32_t kTypes = kBf16 ? (1u << 7) | (1u << 10) : 0u;
-                constexpr uint32_t kIdescS = make_idesc_f16_f32(kRows, kKeys) | kTypes;
-                constexpr uint32_t kIdescO = make_idesc_f16_f32(kRows, D) | kTypes | (1u << 16);  // B: N contiguous
-                const int ring = Shared ? 0 : s;
-                const uint32_t s_tmem = tmem + s * kKeys, o_tmem = tmem + kTmemO + s * D;
-                const uint32_t q_base = smem_addr(sm.q[Shared ? s : 0]);
-                RingAt<L::kSlots> at;
-                uint32_t q_phase = 0, p_phase = 0;
-                bool ok = true;
-                auto wait = [&](uint64_t *bar, uint32_t parity) {
-                    if (ok && !mbar_wait_bounded(bar, parity, abort_flag)) {
-                        give_up(sm, p.err);
-                        ok = false;
-                    }
-                    return ok;
-                };
-                Walk<Shared> walk;
-                Item it;
-                for (walk.begin(); ok && walk.next(p, it);) {
-                    Span span;
-                    const bool rows = it.token1[s] > it.token0[s];
-                    const bool keys = it.has_keys(s);
-                    if (keys) it.span(s, p.a.args, &span);
-                    if (rows) {
-                        if (!wait(&sm.q_full[Shared ? s : 0], q_phase)) break;
-                        q_phase ^= 1u;
-                    }
-                    uint32_t more = 0;
-                    for (int i = it.first[s]; ok && i < it.last[s]; ++i) {
-                        const bool take = keys && span.tile_some(it.key_tile(i) * kKeys);
-                        if (!wait(&sm.full[ring][at.slot], at.parity)) break;
-                        if (take) {
-                            tc_fence_after();
-                            const uint32_t k_base = smem_addr(sm.kv[ring][at.slot]);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == kSoftmaxWarps) {
+            // -------------------------------------------------------------------- products
+            // One warp issues for both streams, stream 0's second product and next scores before
+            // stream 1's: that keeps the streams half a tile apart, so that one's exponentials run while the
+            // other's products do.  (With a thread a stream both ran in step, each waiting for the tensor
+            // core and then for the exponentials at the same time.)
+            constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+            constexpr uint32_t kTypes = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t kIdescS = make_idesc_f16_f32(kRows, kKeys) | kTypes;
+            constexpr uint32_t kIdescO = make_idesc_f16_f32(kRows, D) | kTypes | (1u << 16);  // B: N contiguous
+            constexpr int kLastRing = L::kRings - 1;
+            RingAt<L::kSlots> at[L::kRings];
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            const uint32_t issue = elect_one();
+            uint64_t q_desc[2], k_desc[L::kRings], v_desc[L::kRings];
 #pragma unroll
-                            for (int d = 0; d < D; d += 16) {
-                                const uint32_t off = (d / 64) * (kKeys * 128) + (d % 64) * 2;
-                                umma_f16_ss(s_tmem, make_sw128_kmajor_desc(q_base + off),
-                                            make_sw128_kmajor_desc(k_base + off), kIdescS, d != 0);
-                            }
-                            umma_commit(&sm.s_full[s]);
-                            umma_commit(&sm.empty[ring][at.slot]);
-                        } else {
-                            mbar_arrive(&sm.empty[ring][at.slot]);
-                        }
-                        at.advance();
-                        if (!wait(&sm.full[ring][at.slot], at.parity)) break;
-                        if (take) {
-                            if (!wait(&sm.p_full[s], p_phase)) break;
-                            p_phase ^= 1u;
-                            tc_fence_after();
-                            const uint32_t v_base = smem_addr(sm.kv[ring][at.slot]);
+            for (int s = 0; s < 2; ++s) q_desc[s] = make_sw128_kmajor_desc(smem_addr(sm.q[Shared ? s : 0]));
 #pragma unroll
-                            for (int k = 0; k < kKeys; k += 16) {
-                                umma_f16_ts(o_tmem, s_tmem + k / 2, make_sw128_mnmajor_desc(v_base + k * 128, kKeys * 128),
-                                            kIdescO, more);
-                                more = 1;
-                            }
-                            umma_commit(&sm.empty[ring][at.slot]);
-                        } else {
-                            mbar_arrive(&sm.empty[ring][at.slot]);
-                        }
-                        at.advance();
+            for (int r = 0; r < L::kRings; ++r) {
+                k_desc[r] = make_sw128_kmajor_desc(smem_addr(sm.kv[r][0]));
+                v_desc[r] = make_sw128_mnmajor_desc(smem_addr(sm.kv[r][0]), kKeys * 128);
+            }
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+                if (!ok && lane == 0) give_up(sm, p.err);
+                return ok;
+            };
+            Walk<Shared> walk0(0), walk1(1);
+            Item item[2];
+            while (ok && walk0.next(p, item[0]) && walk1.next(p, item[1])) {
+                const int count[2] = {item[0].last - item[0].first, item[1].last - item[1].first};
+                const int steps = max(count[0], count[1]);
+                uint32_t more[2] = {0, 0}, takes[2] = {0, 0}, took[2] = {0, 0};
+                // Step i: the second product of tile i, then the scores of tile i + 1.
+                for (int i = -1; ok && i < steps; ++i) {
+                    if (((i + 1) & 31) == 0) {  // bit j: whether a stream takes tile i + 1 + j of its list
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) takes[s] = item[s].takes(i + 1, lane, p.a.args);
                     }
-                    // Once an item, with or without products: the softmax warpgroup moves on only after it,
-                    // so no barrier of the item runs a phase ahead of this thread.
-                    if (ok && rows) {
-                        umma_commit(&sm.o_full[s]);
-                        if (!Shared && s == 1) umma_commit(&sm.q_free);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        constexpr int kSlotDesc = L::kTileBytes >> 4;
+                        const int r = s < kLastRing ? s : kLastRing;
+                        const bool release = !Shared || s == 1;  // the last to read the tile
+                        const uint32_t s_tmem = tmem + s * kKeys, o_tmem = tmem + kTmemO + s * D;
+                        const bool take = takes[s] >> ((i + 1) & 31) & 1u;
+                        RingAt<L::kSlots> here = at[r];
+                        if (i < 0 && item[s].rows() && (Shared || s == 0)) {
+                            if (!wait(&sm.q_full[s], q_phase[s])) break;
+                            q_phase[s] ^= 1u;
+                        }
+                        if (i >= 0 && i < count[s]) {
+                            if (!wait(&sm.full[r][here.slot], here.parity)) break;
+                            if (took[s]) {
+                                if (!wait(&sm.p_full[s], p_phase[s])) break;
+                                p_phase[s] ^= 1u;
+                                tc_fence_after();
+                                const uint64_t desc = v_desc[r] + static_cast<uint32_t>(here.slot * kSlotDesc);
+#pragma unroll
+                                for (int k = 0; k < kKeys; k += 16) {
+                                    umma_f16_ts_if(issue, o_tmem, s_tmem + k / 2, desc + (k * 128 >> 4), kIdescO, more[s]);
+                                    more[s] = 1;
+                                }
+                            }
+                            if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
+                            here.advance();
+                        }
+                        if (i + 1 < count[s]) {
+                            if (!wait(&sm.full[r][here.slot], here.parity)) break;
+                            if (take) {
+                                tc_fence_after();
+                                const uint64_t desc = k_desc[r] + static_cast<uint32_t>(here.slot * kSlotDesc);
+#pragma unroll
+                                for (int d = 0; d < D; d += 16) {
+                                    const uint32_t off = ((d / 64) * (kKeys * 128) + (d % 64) * 2) >> 4;
+                                    umma_f16_ss_if(issue, s_tmem, q_desc[s] + off, desc + off, kIdescS, d != 0);
+                                }
+                                umma_commit_if(issue, &sm.s_full[s]);
+                            }
+                            if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
+                            here.advance();
+                        }
+                        if (i + 1 == count[s] && item[s].rows()) {
+                            // Once an item, with or without products: the softmax warpgroup moves on only after
+                            // it, so no barrier of the item runs a phase ahead of this warp.
+                            umma_commit_if(issue, &sm.o_full[s]);
+                            if (!Shared && s == 1) umma_commit_if(issue, &sm.q_free);
+                        }
+                        took[s] = take;
+                        if (release) at[r] = here;
                     }
                 }
-                // Every product issued has ended before the block lets go of its memory.
-                umma_commit(&sm.drain[s]);
-                mbar_wait_bounded(&sm.drain[s], 0, nullptr);
             }
-        } else if (s < L::kRings) {
+            // Every product issued has ended before the block lets go of its memory.
+            umma_commit_if(issue, &sm.drain);
+            mbar_wait_bounded(&sm.drain, 0, nullptr);
+            __syncwarp();
+        } else if (warp >= kSoftmaxWarps + 2 && warp < kSoftmaxWarps + 2 + L::kRings) {
+            const int s = warp - (kSoftmaxWarps + 2);
             // -------------------------------------------------------------------- loads of ring s
             RingAt<L::kSlots> at;
             uint32_t loaded = 0;
             const int groups = kKeys / p.box_rows, boxes = groups * (D / 64);
             bool ok = true;
-            Walk<Shared> walk;
+            Walk<Shared> walk(s);
             Item it;
-            for (walk.begin(); ok && walk.next(p, it);) {
-                for (int i = it.first[s]; ok && i < it.last[s]; ++i) {
+            while (ok && walk.next(p, it)) {
+                for (int i = it.first; ok && i < it.last; ++i) {
                     // Box b of a tile: keys [group * box_rows, ...) and 64 elements.
                     const int group = lane % groups, half = lane / groups;
                     const int key = it.key_tile(i) * kKeys + group * p.box_rows;
@@ -462,7 +485,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---------------------------------------------------------------------- softmax of stream s
         const int s = warp >> 2;
         const int row = threadIdx.x & (kRows - 1);
@@ -480,14 +503,20 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             if (!ok && lane == 0) give_up(sm, p.err);
             return ok;
         };
-        Walk<Shared> walk;
-        Item it;
-        for (walk.begin(); ok && walk.next(p, it); ++item_number) {
-            const bool rows = it.token1[s] > it.token0[s];
-            const bool keys = it.has_keys(s);
-            const int token = it.token0[s] + row_token;
+        Walk<Shared> walk(s);
+        const Item &it = sm.item[warp];
+        for (;; ++item_number) {
+            {
+                Item next;
+                if (!ok || !walk.next(p, next)) break;
+                __syncwarp();
+                if (lane == 0) sm.item[warp] = next;
+                __syncwarp();
+            }
+            const bool rows = it.rows();
+            const int token = it.token0 + row_token;
             const int head = it.kv_head * p.ratio + row_head;
-            const bool valid = row_used && token < it.token1[s];
+            const bool valid = row_used && token < it.token1;
             if (rows && (Shared || s == 0)) {
                 if (!Shared && q_loaded) {  // the other stream's products have read the last tile
                     if (!wait(&sm.q_free, free_phase)) break;
@@ -503,8 +532,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     const int r = (i * kRows + row) / kPacks, e = (row % kPacks) * 8;
                     const int rt = r / p.ratio, rh = r - rt * p.ratio;
                     v[i] = make_uint4(0, 0, 0, 0);
-                    if (rt < p.tile_tokens && it.token0[s] + rt < it.token1[s])
-                        v[i] = *reinterpret_cast<const uint4 *>(q + (it.start + it.token0[s] + rt) * p.a.q.token_stride +
+                    if (rt < p.tile_tokens && it.token0 + rt < it.token1)
+                        v[i] = *reinterpret_cast<const uint4 *>(q + (it.start + it.token0 + rt) * p.a.q.token_stride +
                                                                 (it.kv_head * p.ratio + rh) * p.a.q.head_stride + e);
                 }
 #pragma unroll
@@ -523,23 +552,31 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&sm.q_full[s]);
             }
-            Span span;
-            if (keys) it.span(s, p.a.args, &span);
-            const Visible seen = visible_keys(it.position(token), it.length, p.a.args.window, p.a.args.sinks, p.a.args.frame);
-            const int seen_first = static_cast<int>(seen.first), seen_low = static_cast<int>(seen.low),
-                      seen_high = static_cast<int>(seen.high);
+            int seen_first, seen_low, seen_high;
+            {
+                const Visible seen = visible_keys(it.position(token), it.length, p.a.args.window, p.a.args.sinks, p.a.args.frame);
+                seen_first = static_cast<int>(seen.first);
+                seen_low = static_cast<int>(seen.low);
+                seen_high = static_cast<int>(seen.high);
+            }
             const bool warp_used = __any_sync(0xffffffffu, valid);
             float m = -INFINITY, l = 0.0f;
             bool any = false;
-            for (int i = it.first[s]; i < it.last[s]; ++i) {
-                const int base = it.key_tile(i) * kKeys;
-                if (!(keys && span.tile_some(base))) {
-                    at.advance();
+            uint32_t takes = 0, cuts = 0;
+            for (int i = 0, count = it.last - it.first; i < count; ++i, takes >>= 1, cuts >>= 1) {
+                if ((i & 31) == 0) {
+                    takes = it.takes(i, lane, p.a.args);
+                    cuts = it.cuts(i, lane, p.a.args);
+                }
+                at.advance();  // from the keys' slot to the values'
+                if (!(takes & 1u)) {
                     at.advance();
                     continue;
                 }
-                at.advance();  // the values' slot
-                if (!span.tile_all(base)) {
+                const bool cut = cuts & 1u;
+                if (cut) {
+                    const Span span = it.span(p.a.args);
+                    const int base = it.key_tile(it.first + i) * kKeys;
                     // Some rows' weights are 0 for some keys here, and 0 x non-finite is not 0.  A key that
                     // no row of the block sees becomes zeros; where only some see it, all rows are done alone.
                     if (!wait(&sm.full[ring][at.slot], at.parity)) break;
@@ -571,9 +608,9 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     for (int k = 0; k < kKeys; k += 32) tmem_ld_32x32b_x32(s_tmem + k, x + k);
 #pragma unroll
                     for (int k = 0; k < kKeys; k += 32) tmem_wait_ld_x32(x + k);
-                    const bool clear = !valid || base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high);
-                    if (!__all_sync(0xffffffffu, clear)) {
-                        if (!clear) {
+                    if (cut) {
+                        const int base = it.key_tile(it.first + i) * kKeys;
+                        if (valid && !(base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high))) {
                             const int a = seen_first - base, lo = seen_low - base, hi = seen_high - base;
 #pragma unroll
                             for (int k = 0; k < kKeys; ++k)
@@ -597,14 +634,14 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         const float shrink = to == -INFINITY ? 1.0f : exp2_approx((m - to) * p.c);
                         m = to;
                         l *= shrink;
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 16) {  // 16 columns: the scores hold 128 registers
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_tmem + d, o);
+                            tmem_wait_ld_x16(o);
 #pragma unroll
-                        for (int d = 0; d < D; d += 32) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(o_tmem + d, o);
-                            tmem_wait_ld_x32(o);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                            tmem_st_32x32b_x32_wait(o_tmem + d, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                            tmem_st_32x32b_x16_wait(o_tmem + d, o);
                         }
                     }
                     const float mc = m == -INFINITY ? 0.0f : m * p.c;
@@ -634,11 +671,11 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             tc_fence_after();
             const bool alone = *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) == item_number;
             const int64_t at_row = static_cast<int64_t>(it.start + token) * p.a.args.q_heads + head;
-            const int64_t part_row = static_cast<int64_t>(it.part[s]) * p.a.args.tokens * p.a.args.q_heads + at_row;
+            const int64_t part_row = static_cast<int64_t>(it.part) * p.a.args.tokens * p.a.args.q_heads + at_row;
             T *out = static_cast<T *>(p.a.out.data) + (it.start + token) * p.a.out.token_stride + head * p.a.out.head_stride;
             if (alone) {
                 if (valid)
-                    row_alone<T, D>(p, it, it.first[s], it.last[s], token, head, seen, out,
+                    row_alone<T, D>(p, it, token, head, Visible{seen_first, seen_low, seen_high}, out,
                                     p.part_o ? p.part_o + part_row * D : nullptr, p.part_ml ? p.part_ml + part_row : nullptr);
                 continue;
             }
@@ -834,7 +871,7 @@ cudaError_t prepare() {
     cudaFuncAttributes attr;
     e = cudaFuncGetAttributes(&attr, fn);
     if (e != cudaSuccess) return e;
-    // The softmax warps grow to 224 registers out of what the block starts with (8 x 224 + 4 x 56 = 12 x 168).
+    // The softmax warps grow to 216 registers out of what the block starts with (8 x 216 + 4 x 72 = 12 x 168).
     if (attr.maxThreadsPerBlock < kThreads || attr.numRegs < 168) return cudaErrorInvalidConfiguration;
     return cudaSuccess;
 }
@@ -872,6 +909,7 @@ cudaError_t token_attention_prepare_device() {
 cudaError_t launch_token_attention_tensor(const AttentionParams &a, void *workspace, int sm_count, uint32_t *err,
                                           cudaStream_t stream) {
     const Plan plan = make_plan(a.cache, a.args);
+    if (plan.items >= (int64_t{1} << 30)) return cudaErrorInvalidConfiguration;
     KernelParams k{};
     k.a = a;
     if (plan.parts > 0) {
@@ -884,7 +922,7 @@ cudaError_t launch_token_attention_tensor(const AttentionParams &a, void *worksp
     k.row_blocks = plan.row_blocks;
     k.splits = plan.splits;
     k.box_rows = box_rows(a.cache.page_size);
-    k.items = plan.items;
+    k.items = static_cast<int>(plan.items);
     // Above zero, so that a hidden key's score of -inf stays -inf; 1e-30 makes every weight 1 as 0 would.
     const float c = fabsf(a.args.scale) * 1.4426950408889634f;
     k.c = c > 1e-30f ? c : 1e-30f;
