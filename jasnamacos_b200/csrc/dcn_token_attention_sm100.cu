@@ -181,9 +181,10 @@ struct alignas(1024) Smem {
     uint8_t q[L::kQTiles][L::kTileBytes];
     uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
     uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
-    uint64_t q_full[2], q_free, s_full[2], p_full[2], o_full[2], scanned[2], drain;
-    // Each softmax warp's current item, kept here: the 128 scores of a row need the registers.
-    Item item[kSoftmaxWarps];
+    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], o_full[2], scanned[2], drain;
+    // The current item of each softmax warp and of the product warp's two streams, kept here: the 128
+    // scores of a row need the registers.
+    Item item[kSoftmaxWarps + 2];
     int dirty[2][2];
     int abort_flag;
     uint32_t tmem_base;
@@ -206,6 +207,30 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two FP32 values in one register pair, and the instructions that take two at a time.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 template <typename T>
@@ -317,7 +342,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.q_full[s], kRows);
             mbar_init(&sm.s_full[s], 1);
-            mbar_init(&sm.p_full[s], 4);
+            mbar_init(&sm.p_full[s][0], 4);
+            mbar_init(&sm.p_full[s][1], 4);
             mbar_init(&sm.o_full[s], 1);
             mbar_init(&sm.scanned[s], 4);
             sm.dirty[s][0] = sm.dirty[s][1] = -1;
@@ -365,13 +391,49 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             }
             bool ok = true;
             auto wait = [&](uint64_t *bar, uint32_t parity) {
+                if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
                 if (!ok && lane == 0) give_up(sm, p.err);
                 return ok;
             };
+            auto second = [&](int s, int r, int slot, uint32_t &more) {  // O += P V, half a tile's keys at a time
+                const uint64_t desc = v_desc[r] + static_cast<uint32_t>(slot * (L::kTileBytes >> 4));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!wait(&sm.p_full[s][h], p_phase[s])) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = h * kKeys / 2; k < (h + 1) * kKeys / 2; k += 16) {
+                        umma_f16_ts_if(issue, tmem + kTmemO + s * D, tmem + s * kKeys + k / 2, desc + (k * 128 >> 4), kIdescO,
+                                       more);
+                        more = 1;
+                    }
+                }
+                p_phase[s] ^= 1u;
+                return true;
+            };
+            auto scores = [&](int s, int r, int slot) {  // S = Q K^T
+                const uint64_t desc = k_desc[r] + static_cast<uint32_t>(slot * (L::kTileBytes >> 4));
+#pragma unroll
+                for (int d = 0; d < D; d += 16) {
+                    const uint32_t off = ((d / 64) * (kKeys * 128) + (d % 64) * 2) >> 4;
+                    umma_f16_ss_if(issue, tmem + s * kKeys, q_desc[s] + off, desc + off, kIdescS, d != 0);
+                }
+                umma_commit_if(issue, &sm.s_full[s]);
+            };
             Walk<Shared> walk0(0), walk1(1);
-            Item item[2];
-            while (ok && walk0.next(p, item[0]) && walk1.next(p, item[1])) {
+            const Item *item = sm.item + kSoftmaxWarps;
+            while (ok) {
+                {
+                    Item next[2];
+                    if (!walk0.next(p, next[0]) || !walk1.next(p, next[1])) break;
+                    __syncwarp();
+                    if (lane == 0) {
+                        sm.item[kSoftmaxWarps] = next[0];
+                        sm.item[kSoftmaxWarps + 1] = next[1];
+                    }
+                    __syncwarp();
+                }
                 const int count[2] = {item[0].last - item[0].first, item[1].last - item[1].first};
                 const int steps = max(count[0], count[1]);
                 uint32_t more[2] = {0, 0}, takes[2] = {0, 0}, took[2] = {0, 0};
@@ -381,13 +443,36 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
 #pragma unroll
                         for (int s = 0; s < 2; ++s) takes[s] = item[s].takes(i + 1, lane, p.a.args);
                     }
+                    // The step in the middle of a run of tiles that both streams take, without the general step's
+                    // questions: this warp's instructions between two products are on every tile's path.
+                    while (took[0] & took[1] & takes[0] & takes[1] & (((i + 1) & 31) != 31)) {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const int r = s < kLastRing ? s : kLastRing;
+                            RingAt<L::kSlots> here = at[r];
+                            if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
+                            if (!second(s, r, here.slot, more[s])) break;
+                            if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
+                            here.advance();
+                            if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
+                            scores(s, r, here.slot);
+                            if (!Shared || s == 1) {
+                                umma_commit_if(issue, &sm.empty[r][here.slot]);
+                                here.advance();
+                                at[r] = here;
+                            }
+                        }
+                        if (!ok) break;
+                        ++i;
+                        takes[0] >>= 1;
+                        takes[1] >>= 1;
+                    }
+                    if (!ok) break;
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        constexpr int kSlotDesc = L::kTileBytes >> 4;
                         const int r = s < kLastRing ? s : kLastRing;
                         const bool release = !Shared || s == 1;  // the last to read the tile
-                        const uint32_t s_tmem = tmem + s * kKeys, o_tmem = tmem + kTmemO + s * D;
-                        const bool take = takes[s] >> ((i + 1) & 31) & 1u;
+                        const bool take = takes[s] & 1u;
                         RingAt<L::kSlots> here = at[r];
                         if (i < 0 && item[s].rows() && (Shared || s == 0)) {
                             if (!wait(&sm.q_full[s], q_phase[s])) break;
@@ -395,17 +480,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         }
                         if (i >= 0 && i < count[s]) {
                             if (!wait(&sm.full[r][here.slot], here.parity)) break;
-                            if (took[s]) {
-                                if (!wait(&sm.p_full[s], p_phase[s])) break;
-                                p_phase[s] ^= 1u;
-                                tc_fence_after();
-                                const uint64_t desc = v_desc[r] + static_cast<uint32_t>(here.slot * kSlotDesc);
-#pragma unroll
-                                for (int k = 0; k < kKeys; k += 16) {
-                                    umma_f16_ts_if(issue, o_tmem, s_tmem + k / 2, desc + (k * 128 >> 4), kIdescO, more[s]);
-                                    more[s] = 1;
-                                }
-                            }
+                            if (took[s] && !second(s, r, here.slot, more[s])) break;
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
                         }
@@ -413,13 +488,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             if (!wait(&sm.full[r][here.slot], here.parity)) break;
                             if (take) {
                                 tc_fence_after();
-                                const uint64_t desc = k_desc[r] + static_cast<uint32_t>(here.slot * kSlotDesc);
-#pragma unroll
-                                for (int d = 0; d < D; d += 16) {
-                                    const uint32_t off = ((d / 64) * (kKeys * 128) + (d % 64) * 2) >> 4;
-                                    umma_f16_ss_if(issue, s_tmem, q_desc[s] + off, desc + off, kIdescS, d != 0);
-                                }
-                                umma_commit_if(issue, &sm.s_full[s]);
+                                scores(s, r, here.slot);
                             }
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
@@ -431,6 +500,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             if (!Shared && s == 1) umma_commit_if(issue, &sm.q_free);
                         }
                         took[s] = take;
+                        takes[s] >>= 1;
                         if (release) at[r] = here;
                     }
                 }
@@ -622,10 +692,12 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 4; ++j) top[j] = __uint_as_float(x[j]);
 #pragma unroll
-                    for (int k = 4; k < kKeys; k += 4)
+                    for (int k = 4; k + 8 <= kKeys; k += 8)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[k + j]));
-                    const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        for (int j = 0; j < 4; ++j) top[j] = max3(top[j], __uint_as_float(x[k + j]), __uint_as_float(x[k + 4 + j]));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[kKeys - 4 + j]));
+                    const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]);
                     if (!any) {
                         m = t;
                     } else if (__any_sync(0xffffffffu, (t - m) * p.c > kLag)) {
@@ -645,22 +717,29 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         }
                     }
                     const float mc = m == -INFINITY ? 0.0f : m * p.c;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const uint64_t c2 = pair_of(p.c, p.c), mc2 = pair_of(-mc, -mc);
+                    uint64_t sum[2] = {0, 0};  // two FP32 zeros each
 #pragma unroll
-                    for (int k = 0; k < kKeys; k += 2) {
-                        const float a = exp2_approx(fmaf(__uint_as_float(x[k]), p.c, -mc));
-                        const float b = exp2_approx(fmaf(__uint_as_float(x[k + 1]), p.c, -mc));
-                        sum[k / 2 % 4] += a + b;
-                        x[k / 2] = pack_pair<T>(a, b);
+                    for (int h = 0; h < 2; ++h) {  // the second product starts on the first half's weights
+#pragma unroll
+                        for (int k = h * kKeys / 2; k < (h + 1) * kKeys / 2; k += 2) {
+                            const uint64_t y = fma_pair(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), c2, mc2);
+                            const float a = exp2_approx(low_of(y)), b = exp2_approx(high_of(y));
+                            sum[k / 2 % 2] = add_pair(sum[k / 2 % 2], pair_of(a, b));
+                            x[k / 2] = pack_pair<T>(a, b);
+                        }
+                        tmem_st_32x32b_x32_wait(s_tmem + h * 32, x + h * 32);
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.p_full[s][h]);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st_32x32b_x32_wait(s_tmem, x);
-                    tmem_st_32x32b_x32_wait(s_tmem + 32, x + 32);
-                    tc_fence_before();
-                    __syncwarp();
+                    const uint64_t sums = add_pair(sum[0], sum[1]);
+                    l += low_of(sums) + high_of(sums);
+                } else if (lane == 0) {
+                    mbar_arrive(&sm.p_full[s][0]);
+                    mbar_arrive(&sm.p_full[s][1]);
                 }
                 any = true;
-                if (lane == 0) mbar_arrive(&sm.p_full[s]);
             }
             if (!ok) break;
             if (!rows) continue;
