@@ -433,7 +433,8 @@ dcn_status dcn_forward_f16_static_scratch(const dcn_shape *shape, const void *in
  *
  * Tensors may be strided: a token tensor is [tokens][heads][head_dim] with the strides of dcn_heads
  * (in elements) and unit stride along head_dim.  A token count of zero is a valid call that
- * launches nothing.  Arithmetic is FP32 whatever the element type, rounded once per output. */
+ * launches nothing; a tensor has at most 4096 heads.  Arithmetic is FP32 whatever the element type,
+ * rounded once per output. */
 
 /* A strided [tokens][heads][head_dim] tensor (strides in elements, non-negative). */
 typedef struct dcn_heads {

@@ -184,6 +184,17 @@ __device__ __forceinline__ void bulk_copy_g2s(void *smem_dst, const void *gmem_s
         : "memory");
 }
 
+__device__ __forceinline__ void bulk_copy_s2g(void *gmem_dst, const void *smem_src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gmem_dst), "r"(smem_addr(smem_src)),
+                 "r"(bytes)
+                 : "memory");
+}
+
+// Waits until the bulk stores that this thread issued have read their shared memory.
+__device__ __forceinline__ void bulk_copy_s2g_wait_read() {
+    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *tensor_map, uint64_t *bar,
                                             int c0, int c1, int c2) {
     asm volatile(

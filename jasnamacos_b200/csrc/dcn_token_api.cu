@@ -8,7 +8,7 @@ using namespace dcn;
 namespace {
 
 constexpr int64_t kMaxStride = int64_t{1} << 40;  // elements; every offset then fits 63 bits
-constexpr int32_t kMaxHeads = 65535;
+constexpr int32_t kMaxHeads = 4096;  // of one tensor
 
 size_t element_bytes(int dtype) { return dtype == DCN_DTYPE_F32 ? 4 : 2; }
 
@@ -117,7 +117,7 @@ dcn_status dcn_token_rotary(dcn_dtype dtype, int64_t tokens, int32_t heads, int3
     p.head_dim = head_dim;
     p.tokens = tokens;
     p.rotation = *rotation;
-    return status_from_cuda(launch_token_rotate(dtype, p, reinterpret_cast<cudaStream_t>(stream)));
+    return status_from_cuda(launch_token_rotate(dtype, p, dev.err_word, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const dcn_rotation *rotation,
@@ -166,7 +166,7 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
     p.table_columns = cache->table_columns;
     p.pages = cache->pages;
     p.page_size = cache->page_size;
-    return status_from_cuda(launch_token_rotate(static_cast<dcn_dtype>(cache->dtype), p,
+    return status_from_cuda(launch_token_rotate(static_cast<dcn_dtype>(cache->dtype), p, dev.err_word,
                                                 reinterpret_cast<cudaStream_t>(stream)));
 }
 

@@ -40,7 +40,7 @@ struct RotateParams {
     int32_t streams, table_columns, pages, page_size;
 };
 
-cudaError_t launch_token_rotate(dcn_dtype dtype, const RotateParams &p, cudaStream_t stream);
+cudaError_t launch_token_rotate(dcn_dtype dtype, const RotateParams &p, uint32_t *err, cudaStream_t stream);
 
 struct AttentionParams {
     dcn_paged_cache cache;
@@ -80,11 +80,23 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// VEC elements as one load or store: 16 bytes, or a single element.
+// The register type of one load or store of 2 to 16 bytes.
+template <int Bytes>
+struct Word;
+template <>
+struct Word<2> { using type = uint16_t; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<16> { using type = uint4; };
+
+// VEC elements as one load or store.
 template <typename T, int VEC>
-struct alignas(VEC == 1 ? sizeof(T) : 16) Pack {
-    static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a pack is one element or 16 bytes");
-    T e[VEC];
+struct Pack {
+    using W = typename Word<VEC * static_cast<int>(sizeof(T))>::type;
+    W w;
 };
 
 template <typename T>
@@ -92,26 +104,61 @@ constexpr int kVec = static_cast<int>(16 / sizeof(T));
 
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const Pack<T, VEC> &p, float (&v)[VEC]) {
+    union {
+        typename Pack<T, VEC>::W w;
+        uint16_t h[VEC];
+        float f[VEC];
+    } u;
+    u.w = p.w;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_float<T>(p.e[i]);
+    for (int i = 0; i < VEC; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = u.f[i];
+        else if constexpr (__is_same(T, __half)) v[i] = __half2float(__ushort_as_half(u.h[i]));
+        else v[i] = __uint_as_float(static_cast<uint32_t>(u.h[i]) << 16);
+    }
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> pack(const float (&v)[VEC]) {
-    Pack<T, VEC> p;
+    union {
+        typename Pack<T, VEC>::W w;
+        uint16_t h[VEC];
+        uint32_t hh[(VEC + 1) / 2];
+        float f[VEC];
+    } u;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p.e[i] = from_float<T>(v[i]);
+        for (int i = 0; i < VEC; ++i) u.f[i] = v[i];
+    } else if constexpr (VEC == 1) {
+        const T t = from_float<T>(v[0]);
+        u.h[0] = *reinterpret_cast<const uint16_t *>(&t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            if constexpr (__is_same(T, __half)) {
+                const __half2 t = __floats2half2_rn(v[i], v[i + 1]);
+                u.hh[i / 2] = *reinterpret_cast<const uint32_t *>(&t);
+            } else {
+                const __nv_bfloat162 t = __floats2bfloat162_rn(v[i], v[i + 1]);
+                u.hh[i / 2] = *reinterpret_cast<const uint32_t *>(&t);
+            }
+        }
+    }
+    Pack<T, VEC> p;
+    p.w = u.w;
     return p;
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
-    return *reinterpret_cast<const Pack<T, VEC> *>(p);
+    Pack<T, VEC> v;
+    v.w = *reinterpret_cast<const typename Pack<T, VEC>::W *>(p);
+    return v;
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
-    *reinterpret_cast<Pack<T, VEC> *>(p) = v;
+    *reinterpret_cast<typename Pack<T, VEC>::W *>(p) = v.w;
 }
 
 // ---- streams ---------------------------------------------------------------------------
