@@ -58,6 +58,7 @@ size_t slab_packed_weight_bytes(const Params &p);
 cudaError_t slab_prepare_device();
 cudaError_t temporal_prepare_device();
 cudaError_t token_attention_prepare_device();
+cudaError_t token_norm_prepare_device();
 cudaError_t launch_regroup_slabs(const Params &p, const SplitInput<__half> &input, void *workspace,
                                  cudaStream_t stream);
 cudaError_t launch_prepack_slab(const Params &p, const void *src, dcn_dtype src_dtype, int layout, void *dst,
@@ -151,6 +152,7 @@ dcn_status current_device(DeviceInfo **out) {
             if (e == cudaSuccess) e = slab_prepare_device();
             if (e == cudaSuccess) e = temporal_prepare_device();
             if (e == cudaSuccess) e = token_attention_prepare_device();
+            if (e == cudaSuccess) e = token_norm_prepare_device();
             if (e != cudaSuccess) {
                 cudaGetLastError();
                 return from_cuda(e);

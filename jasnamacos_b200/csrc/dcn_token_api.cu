@@ -218,7 +218,7 @@ dcn_status dcn_token_norm(const dcn_token_norm_args *args, dcn_stream stream) {
     LaunchDevice dev;
     dcn_status st = launch_device(&dev);
     if (st != DCN_OK) return st;
-    return status_from_cuda(launch_token_norm(a, reinterpret_cast<cudaStream_t>(stream)));
+    return status_from_cuda(launch_token_norm(a, dev.err_word, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

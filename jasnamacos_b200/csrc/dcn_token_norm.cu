@@ -15,19 +15,21 @@ namespace dcn {
 namespace {
 
 // The sum of a team's values, in every thread of it: NT threads, one warp or NT / 32 whole warps
-// with the named barrier `team + 1` and the scratch of their own.
+// with the named barrier `team + 1` and scratch of their own.  `scratch` has two halves that take turns: a
+// thread that is at the next sum but one has passed the barrier after all threads read this one.
 template <int NT>
-__device__ __forceinline__ float row_sum(float v, float *scratch, int team) {
+__device__ __forceinline__ float row_sum(float v, float *&scratch, int team) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (NT == 32) return v;
     const int warp = (threadIdx.x % NT) >> 5;
-    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(NT) : "memory");  // the previous sum has been read
     if ((threadIdx.x & 31) == 0) scratch[warp] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(NT) : "memory");
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) s += scratch[w];  // in a fixed order
+    const uint32_t half = NT / 32 * sizeof(float);
+    scratch = reinterpret_cast<float *>(reinterpret_cast<uintptr_t>(scratch) ^ half);
     return s;
 }
 
@@ -36,7 +38,7 @@ struct Row {
     float v[NV][VEC];
 
     // x <- N(x) over `width` elements.  Places past the width hold 0.
-    __device__ __forceinline__ void normalise(int kind, int width, float epsilon, int lane, float *scratch,
+    __device__ __forceinline__ void normalise(int kind, int width, float epsilon, int lane, float *&scratch,
                                               int team) {
         const float inv = 1.0f / static_cast<float>(width);
         if (kind == DCN_NORM_LAYER) {
@@ -66,26 +68,17 @@ struct Row {
     }
 };
 
-// NT threads (a team) hold a row, NV packs of VEC elements each: pack i of thread t covers elements
-// [(i NT + t) VEC, ...).  A block has kTeams teams and takes `block_rows` rows one after another.
-//
-// Shared: the vectors of a modulation group are folded once into FP32 vectors in shared memory --
-//   gate, w (1 + scale), b (1 + scale) + shift, and the post norm's two -- and all of the block's rows of
-// that group read them there.  A row then costs its own loads and stores, three 16-byte shared loads per
-// four elements and some ten instructions an element; without it each row converts and combines up to
-// seven vectors anew, and that, not memory, is what it takes its time on.
-constexpr int kCoefficients = 5;
-enum { kGate = 0, kScale, kShift, kPostWeight, kPostBias };
-
-template <typename T, int VEC, int NT, int NV, int kTeams, bool Shared>
-__global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const dcn_token_norm_args a, int block_rows) {
-    extern __shared__ float folded[];  // [kCoefficients][width], where Shared
-    __shared__ float scratch_of[kTeams][NT / 32];
+// The kernel for any row.  NT threads (a team) hold it, NV packs of VEC elements each: pack i of thread t
+// covers elements [(i NT + t) VEC, ...).  A block has kTeams teams, one row each.
+template <typename T, int VEC, int NT, int NV, int kTeams>
+__global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const __grid_constant__ dcn_token_norm_args a) {
+    __shared__ __align__(2 * NT / 32 * sizeof(float)) float scratch_of[kTeams][2 * NT / 32];
     const int lane = threadIdx.x % NT, team = threadIdx.x / NT;
     float *scratch = scratch_of[team];
     const int width = a.width;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * block_rows;
-    const int64_t end = min(first + block_rows, a.rows);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+    if (row >= a.rows) return;
+    const int64_t group = row / a.group;
 
     auto at = [&](const void *base, int64_t offset) { return static_cast<const T *>(base) + offset; };
     auto vector = [&](const void *base, int64_t offset, float (&v)[VEC], float otherwise) {
@@ -96,73 +89,169 @@ __global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const dcn_token_
             for (int j = 0; j < VEC; ++j) v[j] = otherwise;
         }
     };
-    const bool has_gate = a.gate, has_scale = a.weight || a.scale, has_shift = a.bias || a.shift;
-
-    for (int64_t segment = first; segment < end;) {
-        const int64_t g = segment / a.group;
-        const int64_t segment_end = Shared ? min((g + 1) * a.group, end) : end;
-        if (Shared) {
-            __syncthreads();
-            for (int c = threadIdx.x; c < width; c += NT * kTeams) {
-                auto one = [&](const void *base, int64_t offset, float otherwise) {
-                    return base ? to_float<T>(*at(base, offset + c)) : otherwise;
-                };
-                const float scale = 1.0f + one(a.scale, g * a.scale_stride, 0.0f);
-                folded[kGate * width + c] = one(a.gate, g * a.gate_stride, 1.0f);
-                folded[kScale * width + c] = one(a.weight, 0, 1.0f) * scale;
-                folded[kShift * width + c] = one(a.bias, 0, 0.0f) * scale + one(a.shift, g * a.shift_stride, 0.0f);
-                if (a.post) {
-                    folded[kPostWeight * width + c] = one(a.post_weight, 0, 1.0f);
-                    folded[kPostBias * width + c] = one(a.post_bias, 0, 0.0f);
-                }
-            }
-            __syncthreads();
+    Row<T, VEC, NT, NV> x;
+    Pack<T, VEC> xp[NV], rp[NV];
+    // Both tensors' loads go out before anything waits for either.
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * NT + lane) * VEC;
+        if (c < width) {
+            xp[i] = load_pack<T, VEC>(at(a.x, row * a.x_stride + c));
+            if (a.residual) rp[i] = load_pack<T, VEC>(at(a.residual, row * a.residual_stride + c));
         }
-        auto coefficient = [&](int which, int c, float (&v)[VEC]) {
-            if (VEC % 4 == 0) {
+    }
 #pragma unroll
-                for (int j = 0; j < VEC; j += 4)
-                    *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(folded + which * width + c + j);
-            } else {
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * NT + lane) * VEC;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = folded[which * width + c + j];
-            }
-        };
-        for (int64_t row = segment + team; row < segment_end; row += kTeams) {
-            const int64_t group = Shared ? g : row / a.group;
-            Row<T, VEC, NT, NV> x;
-            Pack<T, VEC> xp[NV], rp[NV];
-            // Both tensors' loads go out before anything waits for either.
+        for (int j = 0; j < VEC; ++j) x.v[i][j] = 0.0f;
+        if (c < width) unpack<T, VEC>(xp[i], x.v[i]);
+    }
+    if (a.residual) {
+        if (a.post) {
+            x.normalise(a.kind, width, a.epsilon, lane, scratch, team);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * NT + lane) * VEC;
                 if (c < width) {
-                    xp[i] = load_pack<T, VEC>(at(a.x, row * a.x_stride + c));
-                    if (a.residual) rp[i] = load_pack<T, VEC>(at(a.residual, row * a.residual_stride + c));
+                    float w[VEC], b[VEC];
+                    vector(a.post_weight, c, w, 1.0f);
+                    vector(a.post_bias, c, b, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], b[j]);
                 }
             }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * NT + lane) * VEC;
+            if (c < width) {
+                float m[VEC], r[VEC];
+                vector(a.gate, group * a.gate_stride + c, m, 1.0f);
+                unpack<T, VEC>(rp[i], r);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], m[j], r[j] * a.residual_scale);
+                if (a.hidden)
+                    store_pack<T, VEC>(static_cast<T *>(a.hidden) + row * a.hidden_stride + c, pack<T, VEC>(x.v[i]));
+            }
+        }
+    }
+    if (a.out == nullptr) return;
+    x.normalise(a.kind, width, a.epsilon, lane, scratch, team);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * NT + lane) * VEC;
+        if (c < width) {
+            float w[VEC], b[VEC];
+            vector(a.weight, c, w, 1.0f);
+            vector(a.bias, c, b, 0.0f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], b[j]);
+            if (a.scale || a.shift) {
+                vector(a.scale, group * a.scale_stride + c, w, 0.0f);
+                vector(a.shift, group * a.shift_stride + c, b, 0.0f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], x.v[i][j]) + b[j];
+            }
+            store_pack<T, VEC>(static_cast<T *>(a.out) + row * a.out_stride + c, pack<T, VEC>(x.v[i]));
+        }
+    }
+}
+
+// The kernel for many rows of up to 128 packs that share their modulation.  A warp holds a row.
+//
+// The vectors of a modulation group are folded once a block into FP32 vectors in shared memory -- gate,
+// w (1 + scale), b (1 + scale) + shift, the post norm's two -- and all of the block's rows of the group read
+// them there; converting and combining up to seven vectors anew for each row takes longer than the row's
+// memory traffic.  A warp's next row lands in shared memory by bulk copies while it works on this one,
+// which costs it no registers.
+enum { kGate = 0, kScale, kShift, kPostWeight, kPostBias };
+
+constexpr int kFoldedWarps = 8;
+constexpr int kFoldedRows = 64;  // rows a block, at least
+constexpr int kStages = 2;       // rows of a warp in shared memory
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(32 * kFoldedWarps) token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a,
+                                                                             int block_rows, uint32_t *err) {
+    constexpr int VEC = kVec<T>;
+    extern __shared__ float4 raw[];
+    __shared__ uint64_t landed[kFoldedWarps][kStages];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int width = a.width, bytes = width * static_cast<int>(sizeof(T));
+    const int coefficients = a.post ? 5 : 3, tensors = a.residual ? 2 : 1;
+    float *folded = reinterpret_cast<float *>(raw);  // [coefficients][width]
+    uint8_t *rows = reinterpret_cast<uint8_t *>(folded + coefficients * width) + warp * kStages * tensors * bytes;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * block_rows;
+    const int64_t end = min(first + block_rows, a.rows);
+
+    auto at = [&](const void *base, int64_t offset) { return static_cast<const T *>(base) + offset; };
+    auto fetch = [&](int64_t row, int stage) {  // one lane's call
+        uint8_t *to = rows + stage * tensors * bytes;
+        mbar_arrive_expect_tx(&landed[warp][stage], tensors * bytes);
+        bulk_copy_g2s(to, at(a.x, row * a.x_stride), bytes, &landed[warp][stage]);
+        if (a.residual) bulk_copy_g2s(to + bytes, at(a.residual, row * a.residual_stride), bytes, &landed[warp][stage]);
+    };
+    int64_t row = first + warp;
+    if (lane == 0) {
+        for (int s = 0; s < kStages; ++s) mbar_init(&landed[warp][s], 1);
+        fence_mbarrier_init();
+        for (int s = 0; s < kStages; ++s)
+            if (row + s * kFoldedWarps < end) fetch(row + s * kFoldedWarps, s);
+    }
+    __syncwarp();
+    auto coefficient = [&](int which, int c, float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4)
+            *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(folded + which * width + c + j);
+    };
+    bool ok = true;
+    float *scratch = nullptr;  // a row is one warp's
+    int stage = 0;
+    uint32_t parity = 0;
+    for (int64_t segment = first; segment < end;) {
+        const int64_t g = segment / a.group;
+        const int64_t segment_end = min((g + 1) * a.group, end);
+        __syncthreads();
+        for (int c = threadIdx.x; c < width; c += 32 * kFoldedWarps) {
+            auto one = [&](const void *base, int64_t offset, float otherwise) {
+                return base ? to_float<T>(*at(base, offset + c)) : otherwise;
+            };
+            const float scale = 1.0f + one(a.scale, g * a.scale_stride, 0.0f);
+            folded[kGate * width + c] = one(a.gate, g * a.gate_stride, 1.0f);
+            folded[kScale * width + c] = one(a.weight, 0, 1.0f) * scale;
+            folded[kShift * width + c] = one(a.bias, 0, 0.0f) * scale + one(a.shift, g * a.shift_stride, 0.0f);
+            if (a.post) {
+                folded[kPostWeight * width + c] = one(a.post_weight, 0, 1.0f);
+                folded[kPostBias * width + c] = one(a.post_bias, 0, 0.0f);
+            }
+        }
+        __syncthreads();
+        for (; row < segment_end; row += kFoldedWarps) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&landed[warp][stage], parity, nullptr));
+            if (!ok) {
+                if (lane == 0) atomicOr(err, kErrWaitTimeout);
+                continue;
+            }
+            const T *here = reinterpret_cast<const T *>(rows + stage * tensors * bytes);
+            Row<T, VEC, 32, NV> x;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * NT + lane) * VEC;
+                const int c = (i * 32 + lane) * VEC;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) x.v[i][j] = 0.0f;
-                if (c < width) unpack<T, VEC>(xp[i], x.v[i]);
+                if (c < width) unpack<T, VEC>(load_pack<T, VEC>(here + c), x.v[i]);
             }
             if (a.residual) {
                 if (a.post) {
-                    x.normalise(a.kind, width, a.epsilon, lane, scratch, team);
+                    x.normalise(a.kind, width, a.epsilon, lane, scratch, 0);
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
-                        const int c = (i * NT + lane) * VEC;
+                        const int c = (i * 32 + lane) * VEC;
                         if (c < width) {
                             float w[VEC], b[VEC];
-                            if (Shared) {
-                                coefficient(kPostWeight, c, w);
-                                coefficient(kPostBias, c, b);
-                            } else {
-                                vector(a.post_weight, c, w, 1.0f);
-                                vector(a.post_bias, c, b, 0.0f);
-                            }
+                            coefficient(kPostWeight, c, w);
+                            coefficient(kPostBias, c, b);
 #pragma unroll
                             for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], b[j]);
                         }
@@ -170,56 +259,35 @@ __global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const dcn_token_
                 }
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int c = (i * NT + lane) * VEC;
+                    const int c = (i * 32 + lane) * VEC;
                     if (c < width) {
                         float m[VEC], r[VEC];
-                        unpack<T, VEC>(rp[i], r);
+                        unpack<T, VEC>(load_pack<T, VEC>(here + width + c), r);
+                        coefficient(kGate, c, m);
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) r[j] *= a.residual_scale;
-                        if (has_gate) {
-                            if (Shared) coefficient(kGate, c, m);
-                            else vector(a.gate, group * a.gate_stride + c, m, 1.0f);
-#pragma unroll
-                            for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], m[j], r[j]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < VEC; ++j) x.v[i][j] += r[j];
-                        }
+                        for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], m[j], r[j] * a.residual_scale);
                         if (a.hidden)
                             store_pack<T, VEC>(static_cast<T *>(a.hidden) + row * a.hidden_stride + c, pack<T, VEC>(x.v[i]));
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0 && row + kStages * kFoldedWarps < end) fetch(row + kStages * kFoldedWarps, stage);
+            if (++stage == kStages) {
+                stage = 0;
+                parity ^= 1u;
+            }
             if (a.out == nullptr) continue;
-            x.normalise(a.kind, width, a.epsilon, lane, scratch, team);
+            x.normalise(a.kind, width, a.epsilon, lane, scratch, 0);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * NT + lane) * VEC;
+                const int c = (i * 32 + lane) * VEC;
                 if (c < width) {
                     float w[VEC], b[VEC];
-                    if (Shared) {
-                        if (has_scale) {
-                            coefficient(kScale, c, w);
+                    coefficient(kScale, c, w);
+                    coefficient(kShift, c, b);
 #pragma unroll
-                            for (int j = 0; j < VEC; ++j) x.v[i][j] *= w[j];
-                        }
-                        if (has_shift) {
-                            coefficient(kShift, c, b);
-#pragma unroll
-                            for (int j = 0; j < VEC; ++j) x.v[i][j] += b[j];
-                        }
-                    } else {
-                        vector(a.weight, c, w, 1.0f);
-                        vector(a.bias, c, b, 0.0f);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], b[j]);
-                        if (a.scale || a.shift) {
-                            vector(a.scale, group * a.scale_stride + c, w, 0.0f);
-                            vector(a.shift, group * a.shift_stride + c, b, 0.0f);
-#pragma unroll
-                            for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], x.v[i][j]) + b[j];
-                        }
-                    }
+                    for (int j = 0; j < VEC; ++j) x.v[i][j] = fmaf(x.v[i][j], w[j], b[j]);
                     store_pack<T, VEC>(static_cast<T *>(a.out) + row * a.out_stride + c, pack<T, VEC>(x.v[i]));
                 }
             }
@@ -228,26 +296,47 @@ __global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const dcn_token_
     }
 }
 
-constexpr int kSharedRows = 64;  // rows a block takes where it folds the vectors
-
 template <typename T, int VEC, int NT, int NV, int kTeams>
 cudaError_t launch(const dcn_token_norm_args &a, cudaStream_t stream) {
-    // Folding pays where a block's rows are mostly of one group and there are enough rows for every SM
-    // to have some blocks; it needs its vectors in the 48 KB every block may have.
-    const size_t smem = static_cast<size_t>(kCoefficients) * a.width * sizeof(float);
-    const bool folds = a.weight || a.bias || a.scale || a.shift || a.gate || a.post;
-    if (folds && a.group >= kSharedRows / 2 && a.rows >= kSharedRows * 296 && smem <= 48 * 1024) {
-        const unsigned blocks = static_cast<unsigned>((a.rows + kSharedRows - 1) / kSharedRows);
-        token_norm_kernel<T, VEC, NT, NV, kTeams, true><<<blocks, NT * kTeams, smem, stream>>>(a, kSharedRows);
-    } else {
-        // One row a team.  Few rows: one team a block, so that they spread over the SMs.
-        if (kTeams > 1 && a.rows < 148 * kTeams)
-            token_norm_kernel<T, VEC, NT, NV, 1, false><<<static_cast<unsigned>(a.rows), NT, 0, stream>>>(a, 1);
-        else
-            token_norm_kernel<T, VEC, NT, NV, kTeams, false>
-                <<<static_cast<unsigned>((a.rows + kTeams - 1) / kTeams), NT * kTeams, 0, stream>>>(a, kTeams);
-    }
+    // Few rows: one team a block, so that they spread over the SMs.
+    if (kTeams > 1 && a.rows < 148 * kTeams)
+        token_norm_kernel<T, VEC, NT, NV, 1><<<static_cast<unsigned>(a.rows), NT, 0, stream>>>(a);
+    else
+        token_norm_kernel<T, VEC, NT, NV, kTeams>
+            <<<static_cast<unsigned>((a.rows + kTeams - 1) / kTeams), NT * kTeams, 0, stream>>>(a);
     return cudaGetLastError();
+}
+
+// Shared memory of the folded kernel.
+size_t folded_bytes(const dcn_token_norm_args &a, size_t element) {
+    return (a.post ? 5 : 3) * sizeof(float) * a.width + kFoldedWarps * kStages * (a.residual ? 2 : 1) * element * a.width;
+}
+
+template <typename T, int NV>
+cudaError_t launch_folded(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
+    // Even shares of the rows for the blocks that are on the GPU at once (three an SM by registers, fewer
+    // by shared memory), so that no round of blocks is left half empty.
+    const size_t smem = folded_bytes(a, sizeof(T));
+    const int64_t per_sm = static_cast<int64_t>(220 * 1024 / (smem + 1024));
+    const int64_t at_once = 148 * (per_sm < 3 ? per_sm : 3);
+    const int64_t rounds = (a.rows + at_once * 256 - 1) / (at_once * 256);
+    int64_t rows = (a.rows + at_once * rounds - 1) / (at_once * rounds);
+    if (rows < kFoldedRows) rows = kFoldedRows;
+    token_norm_folded_kernel<T, NV><<<static_cast<unsigned>((a.rows + rows - 1) / rows), 32 * kFoldedWarps, smem, stream>>>(
+        a, static_cast<int>(rows), err);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t prepare() {
+    const void *kernels[] = {reinterpret_cast<const void *>(token_norm_folded_kernel<T, 1>),
+                             reinterpret_cast<const void *>(token_norm_folded_kernel<T, 2>),
+                             reinterpret_cast<const void *>(token_norm_folded_kernel<T, 4>)};
+    for (const void *fn : kernels) {
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 // Whether every row and vector may be read in 16-byte packs.
@@ -267,11 +356,19 @@ bool vectorised(const dcn_token_norm_args &a) {
 }
 
 template <typename T>
-cudaError_t launch_typed(const dcn_token_norm_args &a, cudaStream_t stream) {
+cudaError_t launch_typed(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
     constexpr int V = kVec<T>;
     if (vectorised<T>(a)) {
         const int packs = a.width / V;
+        // Folding pays where a block's rows are mostly of one group and every SM has some blocks.
+        if (packs <= 128 && a.group >= kFoldedRows / 2 && a.rows >= kFoldedRows * 296) {
+            if (packs <= 32) return launch_folded<T, 1>(a, err, stream);
+            if (packs <= 64) return launch_folded<T, 2>(a, err, stream);
+            return launch_folded<T, 4>(a, err, stream);
+        }
         if (packs <= 32) return launch<T, V, 32, 1, 8>(a, stream);
+        // A row on four warps is the faster the fewer rows there are (2.0 against 3.0 us for 8 of 128 packs).
+        if (packs <= 128 && a.rows < 148 * 8) return launch<T, V, 128, 1, 1>(a, stream);
         if (packs <= 64) return launch<T, V, 32, 2, 8>(a, stream);
         if (packs <= 128) return launch<T, V, 32, 4, 8>(a, stream);
         if (packs <= 512) return launch<T, V, 128, 4, 2>(a, stream);
@@ -284,11 +381,18 @@ cudaError_t launch_typed(const dcn_token_norm_args &a, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_token_norm(const dcn_token_norm_args &a, cudaStream_t stream) {
+cudaError_t token_norm_prepare_device() {
+    cudaError_t e = prepare<float>();
+    if (e == cudaSuccess) e = prepare<__half>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16>();
+    return e;
+}
+
+cudaError_t launch_token_norm(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
     switch (a.dtype) {
-    case DCN_DTYPE_F16: return launch_typed<__half>(a, stream);
-    case DCN_DTYPE_BF16: return launch_typed<__nv_bfloat16>(a, stream);
-    default: return launch_typed<float>(a, stream);
+    case DCN_DTYPE_F16: return launch_typed<__half>(a, err, stream);
+    case DCN_DTYPE_BF16: return launch_typed<__nv_bfloat16>(a, err, stream);
+    default: return launch_typed<float>(a, err, stream);
     }
 }
 

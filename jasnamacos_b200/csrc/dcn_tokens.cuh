@@ -14,7 +14,8 @@ namespace dcn {
 
 // ---- launchers (arguments already validated) ---------------------------------------
 
-cudaError_t launch_token_norm(const dcn_token_norm_args &a, cudaStream_t stream);
+cudaError_t token_norm_prepare_device();  // set-up, once per device and context
+cudaError_t launch_token_norm(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream);
 
 // One strided head tensor that the rotation kernel reads and writes.  With to_cache, the
 // destination is the cache: dst its first page, dst_token_stride unused.

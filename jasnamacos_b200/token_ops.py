@@ -32,8 +32,12 @@ _KINDS = {"rms": _native.DCN_NORM_RMS, "layer": _native.DCN_NORM_LAYER}
 
 
 def _heads(t) -> _native.DcnHeads:
-    stride = t.stride()
-    return _native.DcnHeads(t.data_ptr(), stride[0], stride[1])
+    token, head, _ = t.stride()
+    return _native.DcnHeads(t.data_ptr(), token, head)
+
+
+def _said(name, t, wanted) -> InvalidArgument:
+    return InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}; {wanted} is wanted")
 
 
 class CudaTokenOps:
@@ -49,33 +53,33 @@ class CudaTokenOps:
         if not torch.cuda.is_available():
             raise DeviceUnavailable()
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
+        self._index = self.device.index
 
     # -- checks ------------------------------------------------------------------
+    # Small calls take some microseconds on the GPU, so a call's own Python counts: each check is one
+    # comparison of plain values, and messages are only made where one fails.
     def _dtype(self, t) -> int:
         dtype = _DTYPES.get(t.dtype)
         if dtype is None:
             raise InvalidArgument(f"element type {t.dtype}: float32, float16 or bfloat16 is wanted")
         return dtype
 
-    def _tokens(self, name, t, tokens, heads, head_dim, dtype) -> None:
+    def _tokens(self, name, t, shape, dtype) -> None:
         """A [tokens][heads][head_dim] tensor with unit stride along head_dim on this device."""
-        if t.shape != (tokens, heads, head_dim) or t.dtype != dtype or t.device != self.device:
-            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; "
-                                  f"({tokens}, {heads}, {head_dim}) {dtype} on {self.device} is wanted")
-        if t.stride(2) != 1 and head_dim > 1:
-            raise InvalidArgument(f"{name} needs unit stride along its last dimension")
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index or (t.stride(2) != 1 and shape[2] > 1):
+            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device} with unit stride along the last dimension")
 
-    def _whole(self, name, t, shape, dtype) -> None:
-        """A contiguous tensor of a given shape and type on this device."""
-        if t.shape != shape or t.dtype != dtype or t.device != self.device or not t.is_contiguous():
-            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; a contiguous {tuple(shape)} "
-                                  f"{dtype} tensor on {self.device} is wanted")
+    def _whole(self, name, t, shape, dtype) -> int:
+        """The address of a contiguous tensor of a given shape and type on this device."""
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index or not t.is_contiguous():
+            raise _said(name, t, f"a contiguous {tuple(shape)} {dtype} tensor on {self.device}")
+        return t.data_ptr()
 
     def _call(self, stream, function, *args) -> None:
         """Calls the library on this operator's device and the given or current stream."""
-        index = self.device.index
-        handle = torch.cuda.current_stream(index).cuda_stream if stream is None else stream.cuda_stream
-        if torch.cuda.current_device() == index:
+        index = self._index
+        handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
+        if torch._C._cuda_getDevice() == index:
             status = function(*args, handle or None)
         else:
             with torch.cuda.device(index):
@@ -83,31 +87,39 @@ class CudaTokenOps:
         if status != _native.DCN_OK:
             raise_for_status(status, function.__name__)
 
+    def _new(self, like, stream):
+        """A contiguous tensor like another one, from the memory of the stream that will write it."""
+        if stream is None:
+            return torch.empty(like.shape, dtype=like.dtype, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(like.shape, dtype=like.dtype, device=self.device)
+
     def _rotation(self, positions, frequencies, pairs, interleaved, tokens) -> _native.DcnRotation:
-        pairs = tuple(pairs)
         if len(pairs) != 3 or min(pairs) < 0:
             raise InvalidArgument(f"pairs {pairs}: one count for each of three axes is wanted")
-        self._whole("positions", positions, (tokens, 3), torch.int32)
-        self._whole("frequencies", frequencies, (sum(pairs),), torch.float64)
-        return _native.DcnRotation(frequencies.data_ptr(), positions.data_ptr(), pairs, bool(interleaved))
+        time, row, column = pairs
+        return _native.DcnRotation(self._whole("frequencies", frequencies, (time + row + column,), torch.float64),
+                                   self._whole("positions", positions, (tokens, 3), torch.int32), (time, row, column),
+                                   1 if interleaved else 0)
 
     def _cache(self, k_cache, v_cache, table, starts, lengths) -> _native.DcnPagedCache:
-        if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-            raise InvalidArgument(f"k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
+        shape = k_cache.shape
+        if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
+            raise InvalidArgument(f"k_cache {tuple(shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} "
                                   f"{v_cache.dtype}: two [pages, page_size, heads, head_dim] tensors of one type are wanted")
-        pages, page_size, heads, head_dim = k_cache.shape
-        ks, vs = k_cache.stride(), v_cache.stride()
-        if k_cache.device != self.device or v_cache.device != self.device or ks[3] != 1 or vs[3] != 1:
+        k_page, k_slot, k_head, k_unit = k_cache.stride()
+        v_page, v_slot, v_head, v_unit = v_cache.stride()
+        index = self._index
+        if k_cache.get_device() != index or v_cache.get_device() != index or k_unit != 1 or v_unit != 1:
             raise InvalidArgument(f"k_cache and v_cache need unit stride along head_dim and to be on {self.device}")
-        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or table.stride(1) != 1:
-            raise InvalidArgument(f"table: a [streams, columns] int32 tensor on {self.device} is wanted")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != index or table.stride(1) != 1:
+            raise _said("table", table, f"a [streams, columns] int32 tensor on {self.device}")
+        pages, page_size, heads, head_dim = shape
         streams, columns = table.shape
-        self._whole("starts", starts, (streams + 1,), torch.int32)
-        self._whole("lengths", lengths, (streams,), torch.int32)
         return _native.DcnPagedCache(
-            k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, page_size, heads,
-            head_dim, self._dtype(k_cache), streams, columns, 0, table.stride(0), table.data_ptr(), starts.data_ptr(),
-            lengths.data_ptr())
+            k_cache.data_ptr(), v_cache.data_ptr(), k_page, k_slot, k_head, v_page, v_slot, v_head, pages, page_size, heads,
+            head_dim, self._dtype(k_cache), streams, columns, 0, table.stride(0), table.data_ptr(),
+            self._whole("starts", starts, (streams + 1,), torch.int32), self._whole("lengths", lengths, (streams,), torch.int32))
 
     # -- positions and cache -----------------------------------------------------
     def rotary(self, x, positions, frequencies, pairs, interleaved=False, out=None, stream=None):
@@ -119,16 +131,14 @@ class CudaTokenOps:
         (2j, 2j+1) when `interleaved`, else (j, j + sum(pairs)); elements past them stay.  `out` may be `x`."""
         if x.dim() != 3:
             raise InvalidArgument(f"x is {tuple(x.shape)}; [tokens, heads, head_dim] is wanted")
-        if stream is not None and out is None:
-            with torch.cuda.stream(stream):  # the result belongs to the stream that writes it
-                out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        tokens, heads, head_dim = x.shape
-        self._tokens("x", x, tokens, heads, head_dim, x.dtype)
+        shape = x.shape
+        tokens, heads, head_dim = shape
+        self._tokens("x", x, shape, x.dtype)
         rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
         if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            out = self._new(x, stream)
         else:
-            self._tokens("out", out, tokens, heads, head_dim, x.dtype)
+            self._tokens("out", out, shape, x.dtype)
         self._call(stream, self.lib.dcn_token_rotary, self._dtype(x), tokens, heads, head_dim, rotation, _heads(x),
                    _heads(out))
         return out
@@ -146,8 +156,9 @@ class CudaTokenOps:
         if k.dim() != 3:
             raise InvalidArgument(f"k is {tuple(k.shape)}; [tokens, kv_heads, head_dim] is wanted")
         tokens, dtype = k.shape[0], k_cache.dtype
-        self._tokens("k", k, tokens, cache.heads, cache.head_dim, dtype)
-        self._tokens("v", v, tokens, cache.heads, cache.head_dim, dtype)
+        _, _, heads, head_dim = k_cache.shape
+        self._tokens("k", k, (tokens, heads, head_dim), dtype)
+        self._tokens("v", v, (tokens, heads, head_dim), dtype)
         rotation = None
         if positions is not None:
             rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
@@ -158,15 +169,11 @@ class CudaTokenOps:
             if q.dim() != 3:
                 raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
             q_heads = q.shape[1]
-            self._tokens("q", q, tokens, q_heads, cache.head_dim, dtype)
+            self._tokens("q", q, (tokens, q_heads, head_dim), dtype)
             if q_out is None:
-                if stream is None:
-                    q_out = torch.empty(q.shape, dtype=dtype, device=self.device)
-                else:
-                    with torch.cuda.stream(stream):
-                        q_out = torch.empty(q.shape, dtype=dtype, device=self.device)
+                q_out = self._new(q, stream)
             else:
-                self._tokens("q_out", q_out, tokens, q_heads, cache.head_dim, dtype)
+                self._tokens("q_out", q_out, (tokens, q_heads, head_dim), dtype)
             q_from, q_to = _heads(q), _heads(q_out)
         elif q_out is not None:
             raise InvalidArgument("q_out needs q")
@@ -186,30 +193,29 @@ class CudaTokenOps:
         if q.dim() != 3:
             raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
         cache = self._cache(k_cache, v_cache, table, starts, lengths)
-        tokens, q_heads, head_dim = q.shape
-        self._tokens("q", q, tokens, q_heads, cache.head_dim, k_cache.dtype)
+        shape = q.shape
+        tokens, q_heads, head_dim = shape
+        self._tokens("q", q, (tokens, q_heads, k_cache.shape[3]), k_cache.dtype)
         args = _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame,
                                              1.0 / math.sqrt(head_dim) if scale is None else scale, 0)
         if out is not None:
-            self._tokens("out", out, tokens, q_heads, head_dim, q.dtype)
+            self._tokens("out", out, shape, q.dtype)
+        else:
+            out = self._new(q, stream)
         need = self.lib.dcn_token_attention_workspace_bytes(cache, args)
-        if stream is None or (out is not None and (workspace is not None or need == 0)):
-            return self._attention(cache, args, q, out, workspace, need, stream)
-        with torch.cuda.stream(stream):
-            return self._attention(cache, args, q, out, workspace, need, stream)
-
-    def _attention(self, cache, args, q, out, workspace, need, stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        given = 0
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        given, address = need, None
         if workspace is not None:
-            if workspace.device != self.device or not workspace.is_contiguous():
-                raise InvalidArgument(f"workspace: contiguous memory on {self.device} is wanted")
-            given = workspace.numel() * workspace.element_size()
-        self._call(stream, self.lib.dcn_token_attention, cache, args, _heads(q), _heads(out),
-                   None if workspace is None else workspace.data_ptr(), given)
+            if workspace.get_device() != self._index or not workspace.is_contiguous():
+                raise _said("workspace", workspace, f"contiguous memory on {self.device}")
+            given, address = workspace.numel() * workspace.element_size(), workspace.data_ptr()
+        elif need:
+            if stream is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            else:
+                with torch.cuda.stream(stream):
+                    workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            address = workspace.data_ptr()
+        self._call(stream, self.lib.dcn_token_attention, cache, args, _heads(q), _heads(out), address, given)
         return out
 
     def attention_workspace_bytes(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0,
@@ -221,26 +227,25 @@ class CudaTokenOps:
 
     # -- norms -------------------------------------------------------------------
     def _vector(self, name, t, width, dtype):
-        if t is None:
-            return None
-        self._whole(name, t, (width,), dtype)
-        return t.data_ptr()
+        return None if t is None else self._whole(name, t, (width,), dtype)
 
     def _modulation(self, name, t, groups, width, dtype):
-        """Pointer and row stride of a [groups, width] tensor with unit stride along its rows."""
+        """Address and row stride of a [groups, width] tensor with unit stride along its rows."""
         if t is None:
             return None, 0
-        if t.dim() != 2 or t.shape[0] < groups or t.shape[1] != width or t.dtype != dtype or t.device != self.device or \
-                (t.stride(1) != 1 and width > 1):
-            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; [{groups}, {width}] {dtype} with unit "
-                                  f"stride along its rows on {self.device} is wanted")
-        return t.data_ptr(), t.stride(0)
+        row, unit = t.stride() if t.dim() == 2 else (0, 0)
+        if t.shape[-1] != width or t.shape[0] < groups or t.dtype != dtype or t.get_device() != self._index or \
+                (unit != 1 and width > 1):
+            raise _said(name, t, f"[{groups}, {width}] {dtype} on {self.device} with unit stride along its rows")
+        return t.data_ptr(), row
 
-    def _rows(self, name, t, shape, dtype) -> int:
-        if t.shape != shape or t.dtype != dtype or t.device != self.device or (t.stride(1) != 1 and shape[1] > 1):
-            raise InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}; {tuple(shape)} {dtype} with unit stride "
-                                  f"along its rows on {self.device} is wanted")
-        return t.stride(0)
+    def _rows(self, name, t, shape, dtype):
+        """Address and row stride of a [rows, width] tensor with unit stride along its rows."""
+        if t is None:
+            return None, 0
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index or (t.stride(1) != 1 and shape[1] > 1):
+            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device} with unit stride along its rows")
+        return t.data_ptr(), t.stride(0)
 
     def _norm(self, x, residual, post, post_weight, post_bias, gate, residual_scale, kind, weight, bias, scale, shift, group,
               eps, hidden, out, stream):
@@ -255,26 +260,19 @@ class CudaTokenOps:
         if group < 1:
             raise InvalidArgument(f"group {group}: at least one row shares a modulation row")
         groups = -(-rows // group)
+        x_at, x_stride = self._rows("x", x, shape, dtype)
+        residual_at, residual_stride = self._rows("residual", residual, shape, dtype)
+        hidden_at, hidden_stride = self._rows("hidden", hidden, shape, dtype)
+        out_at, out_stride = self._rows("out", out, shape, dtype)
         gate_at, gate_stride = self._modulation("gate", gate, groups, width, dtype)
         scale_at, scale_stride = self._modulation("scale", scale, groups, width, dtype)
         shift_at, shift_stride = self._modulation("shift", shift, groups, width, dtype)
         args = _native.DcnTokenNormArgs(
-            rows, group, width, self._dtype(x), _KINDS[kind], post, eps, residual_scale, x.data_ptr(),
-            None if residual is None else residual.data_ptr(), self._vector("post_weight", post_weight, width, dtype),
-            self._vector("post_bias", post_bias, width, dtype), self._vector("weight", weight, width, dtype),
-            self._vector("bias", bias, width, dtype), gate_at, scale_at, shift_at,
-            None if hidden is None else hidden.data_ptr(), out.data_ptr(), self._rows("x", x, shape, dtype),
-            0 if residual is None else self._rows("residual", residual, shape, dtype),
-            0 if hidden is None else self._rows("hidden", hidden, shape, dtype), self._rows("out", out, shape, dtype),
-            gate_stride, scale_stride, shift_stride)
+            rows, group, width, self._dtype(x), _KINDS[kind], post, eps, residual_scale, x_at, residual_at,
+            self._vector("post_weight", post_weight, width, dtype), self._vector("post_bias", post_bias, width, dtype),
+            self._vector("weight", weight, width, dtype), self._vector("bias", bias, width, dtype), gate_at, scale_at, shift_at,
+            hidden_at, out_at, x_stride, residual_stride, hidden_stride, out_stride, gate_stride, scale_stride, shift_stride)
         self._call(stream, self.lib.dcn_token_norm, args)
-
-    @staticmethod
-    def _new(x, stream):
-        if stream is None:
-            return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with torch.cuda.stream(stream):
-            return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
     def norm(self, x, kind="rms", weight=None, bias=None, scale=None, shift=None, group=None, eps=1e-6, out=None, stream=None):
         """The norm before a block: ``(N(x) * weight + bias) * (1 + scale[g]) + shift[g]`` for the rows of

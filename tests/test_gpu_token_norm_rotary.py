@@ -66,6 +66,34 @@ def test_residual_norm(ops, dtype, kind, post, rows, width, group):
     ref.check(out, *want_out)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("width,group,post", [(64, 1000, False), (512, 47, True), (1000, 64, False), (1024, 256, True)])
+def test_residual_norm_of_many_rows(ops, dtype, kind, width, group, post):
+    """Enough rows for the kernel that folds a group's vectors once a block; groups that end inside a block."""
+    rows = 20011
+    g = generator(width + group)
+    groups = -(-rows // group)
+    x, residual = normal(g, (rows, width), dtype, 2.0) - 0.5, normal(g, (rows, width), dtype, 3.0)
+    shift, scale, gate = normal(g, (groups, 3, width), dtype, 0.4).unbind(1)
+    args = dict(gate=gate, residual_scale=1.25, kind=kind, weight=1 + normal(g, (width,), dtype, 0.1), scale=scale, shift=shift,
+                group=group, bias=normal(g, (width,), dtype, 0.1))
+    if post:
+        args |= dict(post_weight=1 + normal(g, (width,), dtype, 0.1), post_bias=normal(g, (width,), dtype, 0.1))
+    hidden, out = ops.residual_norm(x, residual, **args)
+    want_hidden, want_out = ref.norm(x, residual, **args)
+    ref.check(hidden, *want_hidden)
+    ref.check(out, *want_out)
+    again = x.clone()
+    ops.residual_norm(again, residual, **args, hidden=residual, out=again)  # in place
+    assert torch.equal(residual, hidden) and torch.equal(again, out)
+    ref.check(ops.norm(x, kind=kind, weight=args["weight"]), *ref.norm(x, kind=kind, weight=args["weight"])[1])
+    spoiled = x.clone()
+    spoiled[777, 3] = float("nan")
+    clean = torch.arange(rows, device="cuda") != 777
+    assert torch.equal(ops.norm(spoiled, kind=kind)[clean], ops.norm(x, kind=kind)[clean])
+
+
 def test_norm_strides_and_in_place(ops):
     g = generator(5)
     wide = normal(g, (20, 3, 136), F16)
@@ -144,6 +172,30 @@ def test_rotary(ops, dtype, interleaved, tokens, heads, dim, pairs):
     assert torch.equal(ops.rotary(x, at, f, pairs, interleaved=interleaved, out=x), out)  # in place
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,dim,pairs", [
+    (40007, 4, 64, (8, 12, 12)), (20001, 7, 80, (13, 13, 11)), (9000, 6, 128, (16, 22, 22)), (50001, 1, 128, (0, 31, 30)),
+    (3001, 2, 512, (100, 80, 76))])
+def test_rotary_of_many_tokens(ops, dtype, interleaved, tokens, heads, dim, pairs):
+    """Enough rows for the kernel that copies them whole; also from and into strided rows, and in place."""
+    g = generator(tokens + dim)
+    wide = normal(g, (tokens, heads + 2, dim + 16), dtype)
+    at, f = places(g, tokens), series(pairs)
+    x = wide[:, 1:1 + heads, :dim]
+    want, bound = ref.rotary(x, at, f, pairs, interleaved)
+    out = ops.rotary(x, at, f, pairs, interleaved=interleaved)
+    ref.check(out, want, bound)
+    whole = x.contiguous()
+    assert torch.equal(ops.rotary(whole, at, f, pairs, interleaved=interleaved), out)
+    assert torch.equal(ops.rotary(whole, at, f, pairs, interleaved=interleaved, out=whole), out)
+    before = wide.clone()
+    assert ops.rotary(x, at, f, pairs, interleaved=interleaved, out=x) is x
+    assert torch.equal(x, out)
+    assert torch.equal(wide[:, 0], before[:, 0]) and torch.equal(wide[:, -1], before[:, -1])
+    assert torch.equal(wide[:, :, dim:], before[:, :, dim:])
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotary_strides_and_far_positions(ops, interleaved):
     g = generator(3)
@@ -208,6 +260,38 @@ def test_append(ops, dtype, lengths, steps, heads, q_heads, dim, page):
     ref.append(k, v, want_k, want_v, table, starts, have)
     assert ops.append(k, v, k_cache, v_cache, table, starts, have) is None
     assert torch.equal(k_cache, want_k) and torch.equal(v_cache, want_v)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,q_heads,dim,page,pairs", [(4, 8, 128, 64, (16, 24, 24)), (3, 9, 72, 20, (7, 11, 5)),
+                                                          (2, 0, 64, 16, (8, 12, 12))])
+def test_append_of_many_tokens(ops, dtype, heads, q_heads, dim, page, pairs):
+    """Enough rows for the kernel that copies them whole, into a cache with heads before slots as well; a
+    stream without a step, one that has no pages, and padding."""
+    g = generator(dim)
+    lengths, steps = [9000, 4000, 12345, 77, 5000], [9000, 0, 12000, 77, 4999]
+    k_cache, v_cache, table, starts, have = paged(g, lengths, steps, heads, dim, page, dtype)
+    table[3] = -1
+    tokens = sum(steps) + 5
+    qkv = normal(g, (tokens, q_heads + 2 * heads, dim), dtype)
+    q, k, v = qkv.split((q_heads, heads, heads), 1)
+    at, f = places(g, tokens), series(pairs)
+    turned = ops.rotary(qkv, at, f, pairs)
+    want_k, want_v = k_cache.clone(), v_cache.clone()
+    stream = torch.repeat_interleave(torch.arange(5, device="cuda"), torch.tensor(steps, device="cuda"))
+    token = torch.arange(sum(steps), device="cuda")
+    position = have.long()[stream] - starts.long()[stream + 1] + token
+    pages = table[stream, position // page].long()
+    stored = pages >= 0
+    want_k[pages[stored], (position % page)[stored]] = turned[token[stored], q_heads:q_heads + heads]
+    want_v[pages[stored], (position % page)[stored]] = v[token[stored]]
+    for k_to, v_to in ((k_cache.clone(), v_cache.clone()),
+                       (k_cache.transpose(1, 2).contiguous().transpose(1, 2), v_cache.transpose(1, 2).contiguous().transpose(1, 2))):
+        out = ops.append(k, v, k_to, v_to, table, starts, have, q=q if q_heads else None, positions=at, frequencies=f, pairs=pairs)
+        assert torch.equal(k_to, want_k) and torch.equal(v_to, want_v)
+        if q_heads:
+            assert torch.equal(out, turned[:, :q_heads])
+    assert ops.lib.dcn_device_error() == 0
 
 
 def test_append_leaves_out_what_has_no_place(ops):
