@@ -90,9 +90,9 @@ class CudaTokenOps:
     def _new(self, like, stream):
         """A contiguous tensor like another one, from the memory of the stream that will write it."""
         if stream is None:
-            return torch.empty(like.shape, dtype=like.dtype, device=self.device)
+            return like.new_empty(like.shape)
         with torch.cuda.stream(stream):
-            return torch.empty(like.shape, dtype=like.dtype, device=self.device)
+            return like.new_empty(like.shape)
 
     def _rotation(self, positions, frequencies, pairs, interleaved, tokens) -> _native.DcnRotation:
         if len(pairs) != 3 or min(pairs) < 0:
@@ -210,10 +210,10 @@ class CudaTokenOps:
             given, address = workspace.numel() * workspace.element_size(), workspace.data_ptr()
         elif need:
             if stream is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+                workspace = q.new_empty(need, dtype=torch.uint8)
             else:
                 with torch.cuda.stream(stream):
-                    workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+                    workspace = q.new_empty(need, dtype=torch.uint8)
             address = workspace.data_ptr()
         self._call(stream, self.lib.dcn_token_attention, cache, args, _heads(q), _heads(out), address, given)
         return out
