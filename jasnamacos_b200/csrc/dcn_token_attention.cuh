@@ -16,7 +16,8 @@ struct Visible {
 __host__ __device__ inline Visible visible_keys(int64_t position, int64_t length, int window, int sinks, int frame) {
     Visible v{0, 0, 0};
     if (position < 0 || length <= 0) return v;
-    const int64_t own = position / frame;
+    // Positions are below 2^31: a 32-bit division (a 64-bit one is a routine of a hundred instructions).
+    const int64_t own = static_cast<uint32_t>(position) / static_cast<uint32_t>(frame);
     const int64_t end = (own + 1) * frame;
     v.high = end < length ? end : length;
     const int64_t start = (own - window + 1) * frame;

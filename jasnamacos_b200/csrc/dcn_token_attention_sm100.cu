@@ -55,6 +55,7 @@ struct KernelParams {
     float2 *part_ml;     // [parts][tokens][q_heads] (c m, l)
     uint32_t *err;
     int ratio;           // query heads of a key head
+    int per_ratio;       // 2^16 / ratio, rounded up: r * per_ratio >> 16 is r / ratio for a tile's rows
     int tile_tokens;     // tokens of a row tile
     int row_blocks;      // row blocks of the longest step
     int splits;          // blocks that share one row block's keys
@@ -70,7 +71,8 @@ struct Span {
     int pinned, low, high, low_all, high_all;
 
     __device__ __forceinline__ void set(int p0, int p1, int length, const dcn_token_attention_args &a) {
-        const int64_t f0 = p0 / a.frame, f1 = p1 / a.frame;
+        const uint32_t frame = a.frame;
+        const int64_t f0 = static_cast<uint32_t>(p0) / frame, f1 = static_cast<uint32_t>(p1) / frame;
         const int64_t high0 = (f0 + 1) * a.frame, high1 = (f1 + 1) * a.frame;
         const int64_t low0 = (f0 - a.window + 1) * a.frame, low1 = (f1 - a.window + 1) * a.frame;
         high = static_cast<int>(min(high1, static_cast<int64_t>(length)));
@@ -95,6 +97,7 @@ struct Item {
     int stream, kv_head, start, steps, length;  // steps: the stream's tokens of this step
     int token0, token1;             // the tile's tokens in the step
     int first, last;                // range of the list of key tiles
+    int both_last;                  // and the end of both streams' ranges
     int pinned_tiles, window_tile;  // the list: tiles [0, pinned_tiles), then from window_tile
     int part;
     Span both;                      // of the rows of both streams
@@ -132,14 +135,15 @@ struct Walk {
     __device__ __forceinline__ bool next(const KernelParams &p, Item &it) {
         const int block_tokens = p.tile_tokens * (Shared ? 2 : 1);
         while (w < p.items) {
-            int rest = w;
-            const int split = rest % p.splits;
-            rest /= p.splits;
+            uint32_t rest = w;
+            const uint32_t splits = p.splits, row_blocks = p.row_blocks, heads = p.a.cache.heads;
+            const int split = rest % splits;
+            rest /= splits;
             // Later row blocks first: under a causal mask they have the most keys.
-            const int first_block = p.row_blocks - 1 - rest % p.row_blocks;
-            rest /= p.row_blocks;
-            it.kv_head = rest % p.a.cache.heads;
-            it.stream = rest / p.a.cache.heads;
+            const int first_block = row_blocks - 1 - rest % row_blocks;
+            rest /= row_blocks;
+            it.kv_head = rest % heads;
+            it.stream = rest / heads;
             it.start = p.a.cache.starts[it.stream];
             it.steps = p.a.cache.starts[it.stream + 1] - it.start;
             it.length = p.a.cache.lengths[it.stream];
@@ -164,11 +168,12 @@ struct Walk {
                 it.window_tile = max(it.both.low / kKeys, it.pinned_tiles);
                 tiles = it.pinned_tiles + max(0, (it.both.high + kKeys - 1) / kKeys - it.window_tile);
             }
-            const int parts = Shared ? p.splits : 2 * p.splits;
-            const int each = (tiles + parts - 1) / parts;
+            const uint32_t parts = Shared ? splits : 2 * splits;
+            const int each = (static_cast<uint32_t>(tiles) + parts - 1) / parts;
             it.part = Shared ? split : 2 * split + s;
             it.first = min(it.part * each, tiles);
             it.last = min(it.first + each, tiles);
+            it.both_last = Shared ? it.last : min((2 * split + 2) * each, tiles);
             return true;
         }
         return false;
@@ -181,10 +186,11 @@ struct alignas(1024) Smem {
     uint8_t q[L::kQTiles][L::kTileBytes];
     uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
     uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
-    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], o_full[2], scanned[2], drain;
+    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], o_full[2], scanned[2], merge_ready, merge_read, drain;
     // The current item of each softmax warp and of the product warp's two streams, kept here: the 128
     // scores of a row need the registers.
     Item item[kSoftmaxWarps + 2];
+    float2 other_ml[kRows];  // stream 1's (c m, l), where stream 0 merges the two
     int dirty[2][2];
     int abort_flag;
     uint32_t tmem_base;
@@ -350,6 +356,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         }
         mbar_init(&sm.q_free, 1);
         mbar_init(&sm.drain, 1);
+        mbar_init(&sm.merge_ready, 4);
+        mbar_init(&sm.merge_read, 4);
         sm.abort_flag = 0;
         fence_mbarrier_init();
         prefetch_tensor_map(&k_map);
@@ -562,10 +570,10 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         const int ring = Shared ? 0 : s;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + lanes + s * kKeys, o_tmem = tmem + lanes + kTmemO + s * D;
-        const int row_token = row / p.ratio, row_head = row - row_token * p.ratio;
+        const int row_token = row * p.per_ratio >> 16, row_head = row - row_token * p.ratio;
         const bool row_used = row_token < p.tile_tokens;
         RingAt<L::kSlots> at;
-        uint32_t s_phase = 0, item_phase = 0, free_phase = 0;
+        uint32_t s_phase = 0, item_phase = 0, free_phase = 0, merge_phase = 0;
         int item_number = 0;
         bool ok = true, q_loaded = false;
         auto wait = [&](uint64_t *bar, uint32_t parity) {  // the whole warp gives up together
@@ -600,7 +608,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < kPacks; ++i) {
                     const int r = (i * kRows + row) / kPacks, e = (row % kPacks) * 8;
-                    const int rt = r / p.ratio, rh = r - rt * p.ratio;
+                    const int rt = r * p.per_ratio >> 16, rh = r - rt * p.ratio;
                     v[i] = make_uint4(0, 0, 0, 0);
                     if (rt < p.tile_tokens && it.token0 + rt < it.token1)
                         v[i] = *reinterpret_cast<const uint4 *>(q + (it.start + it.token0 + rt) * p.a.q.token_stride +
@@ -748,49 +756,102 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             if (!wait(&sm.o_full[s], item_phase) || !wait(&sm.scanned[s], item_phase)) break;
             item_phase ^= 1u;
             tc_fence_after();
-            const bool alone = *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) == item_number;
+            bool alone = *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) == item_number;
             const int64_t at_row = static_cast<int64_t>(it.start + token) * p.a.args.q_heads + head;
             const int64_t part_row = static_cast<int64_t>(it.part) * p.a.args.tokens * p.a.args.q_heads + at_row;
             T *out = static_cast<T *>(p.a.out.data) + (it.start + token) * p.a.out.token_stride + head * p.a.out.head_stride;
-            if (alone) {
-                if (valid)
-                    row_alone<T, D>(p, it, token, head, Visible{seen_first, seen_low, seen_high}, out,
-                                    p.part_o ? p.part_o + part_row * D : nullptr, p.part_ml ? p.part_ml + part_row : nullptr);
+            // Unsplit, the block has all of its rows' keys: stream 0 merges stream 1's sums, and its O from
+            // tensor memory, whose lanes both warpgroups reach.
+            const bool merge = !Shared && p.part_o == nullptr;
+            float2 other = make_float2(-INFINITY, 0.0f);
+            float mc = m * p.c;
+            if (merge && s == 1) {
+                sm.other_ml[row] = any ? make_float2(mc, l) : other;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.merge_ready);
+                if (!wait(&sm.merge_read, merge_phase)) break;  // its O may be written again
+                merge_phase ^= 1u;
                 continue;
             }
-            if (!warp_used) continue;
-            const bool none = seen_first <= 0 && seen_high <= seen_low;
-            if (p.part_o) {
-                if (valid) p.part_ml[part_row] = any ? make_float2(m * p.c, l) : make_float2(-INFINITY, 0.0f);
-                if (!any) continue;  // a part without weight is not read
+            if (merge) {
+                if (!wait(&sm.merge_ready, merge_phase)) break;
+                merge_phase ^= 1u;
+                tc_fence_after();
+                other = sm.other_ml[row];
+                alone |= *reinterpret_cast<volatile int *>(&sm.dirty[1][item_number & 1]) == item_number;
             }
-            const float inv = 1.0f / l;
-#pragma unroll
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[32];
-                if (any) {
-                    tmem_ld_32x32b_x32(o_tmem + d, o);
-                    tmem_wait_ld_x32(o);
-                }
-                if (valid && p.part_o) {
-                    float4 *dst = reinterpret_cast<float4 *>(p.part_o + part_row * D + d);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                             __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
-                } else if (valid) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(out + d);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int n = 0; n < 4; ++n)
-                            w[n] = none ? 0u : pack_pair<T>(__uint_as_float(o[8 * j + 2 * n]) * inv,
-                                                            __uint_as_float(o[8 * j + 2 * n + 1]) * inv);
-                        dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+            if (alone) {
+                if (valid) {
+                    Item all = it;
+                    if (merge) all.last = it.both_last;
+                    row_alone<T, D>(p, all, token, head, Visible{seen_first, seen_low, seen_high}, out,
+                                    p.part_o ? p.part_o + part_row * D : nullptr, p.part_ml ? p.part_ml + part_row : nullptr);
                 }
                 __syncwarp();
+            } else if (warp_used) {
+                const bool none = seen_first <= 0 && seen_high <= seen_low;
+                if (p.part_o && valid) p.part_ml[part_row] = any ? make_float2(mc, l) : make_float2(-INFINITY, 0.0f);
+                if (any || !p.part_o) {  // a part without weight is not read
+                    // Factors of the two streams' O; a stream without weight has none.
+                    const bool two = merge && __any_sync(0xffffffffu, other.x != -INFINITY || other.y != 0.0f);
+                    float mine = 1.0f, theirs = 0.0f;
+                    if (two) {
+                        const float to = fmaxf(any ? mc : -INFINITY, other.x);
+                        const float base = to == -INFINITY ? 0.0f : to;
+                        mine = any ? exp2_approx(mc - base) : 0.0f;
+                        theirs = exp2_approx(other.x - base);
+                        l = l * mine + other.y * theirs;
+                    }
+                    if (!p.part_o) {
+                        const float inv = 1.0f / l;
+                        mine *= inv;
+                        theirs *= inv;
+                    }
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t o[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = 0u;
+                        if (any) {
+                            tmem_ld_32x32b_x32(o_tmem + d, o);
+                            tmem_wait_ld_x32(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * mine);
+                        }
+                        if (two) {
+                            uint32_t b[32];
+                            tmem_ld_32x32b_x32(o_tmem + D + d, b);
+                            tmem_wait_ld_x32(b);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                o[j] = __float_as_uint(fmaf(__uint_as_float(b[j]), theirs, __uint_as_float(o[j])));
+                        }
+                        if (valid && p.part_o) {
+                            float4 *dst = reinterpret_cast<float4 *>(p.part_o + part_row * D + d);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                                     __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+                        } else if (valid) {
+                            uint4 *dst = reinterpret_cast<uint4 *>(out + d);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int n = 0; n < 4; ++n)
+                                    w[n] = none ? 0u : pack_pair<T>(__uint_as_float(o[8 * j + 2 * n]),
+                                                                    __uint_as_float(o[8 * j + 2 * n + 1]));
+                                dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            if (merge) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.merge_read);
             }
         }
     }
@@ -904,13 +965,13 @@ Plan make_plan(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
     plan.splits = 1;
     for (int s = 1; s <= 64 && (s == 1 || s * streams <= tiles); ++s) {
         const int64_t rounds = (blocks * s + kSmCount - 1) / kSmCount;
-        const int64_t cost = rounds * ((tiles + s * streams - 1) / (s * streams) + 3) + (plan.shared && s > 1 ? 6 : 0);
+        const int64_t cost = rounds * ((tiles + s * streams - 1) / (s * streams) + 3) + (s > 1 ? 3 : 0);
         if (cost < best) {
             best = cost;
             plan.splits = s;
         }
     }
-    plan.parts = plan.shared && plan.splits == 1 ? 0 : plan.splits * streams;
+    plan.parts = plan.splits == 1 ? 0 : plan.splits * streams;
     plan.items = blocks * plan.splits;
     return plan;
 }
@@ -997,6 +1058,7 @@ cudaError_t launch_token_attention_tensor(const AttentionParams &a, void *worksp
     }
     k.err = err;
     k.ratio = plan.ratio;
+    k.per_ratio = (65536 + plan.ratio - 1) / plan.ratio;
     k.tile_tokens = plan.tile_tokens;
     k.row_blocks = plan.row_blocks;
     k.splits = plan.splits;
