@@ -109,15 +109,16 @@ struct Item {
     __device__ __forceinline__ bool rows() const { return token1 > token0; }
     // Whether some row of the tile has a position in the stream, and what such rows see.
     __device__ __forceinline__ bool keys() const { return rows() && length > 0 && position(token1 - 1) >= 0; }
-    // Bit j: whether the tile's rows see some key of tile i + j of the block's range (a whole warp's call).
-    __device__ __forceinline__ uint32_t takes(int i, int lane, const dcn_token_attention_args &a) const {
+    // Bit j: whether the tile's rows see some key of tile i + j of the block's range, and (cuts) whether some
+    // of them do not see all of it.  A whole warp's call.
+    __device__ __forceinline__ void look(int i, int lane, const dcn_token_attention_args &a, uint32_t *takes,
+                                         uint32_t *cuts) const {
         const int at = first + i + lane;
-        return __ballot_sync(0xffffffffu, keys() && at < last && span(a).tile_some(key_tile(at) * kKeys));
-    }
-    // Of those, the tiles that some of its rows do not see all of.
-    __device__ __forceinline__ uint32_t cuts(int i, int lane, const dcn_token_attention_args &a) const {
-        const int at = first + i + lane;
-        return __ballot_sync(0xffffffffu, keys() && at < last && !span(a).tile_all(key_tile(at) * kKeys));
+        const bool in = keys() && at < last;
+        const Span seen = span(a);
+        const int base = key_tile(at) * kKeys;
+        *takes = __ballot_sync(0xffffffffu, in && seen.tile_some(base));
+        *cuts = __ballot_sync(0xffffffffu, in && !seen.tile_all(base));
     }
     __device__ __forceinline__ Span span(const dcn_token_attention_args &a) const {
         Span out;
@@ -449,7 +450,10 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 for (int i = -1; ok && i < steps; ++i) {
                     if (((i + 1) & 31) == 0) {  // bit j: whether a stream takes tile i + 1 + j of its list
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) takes[s] = item[s].takes(i + 1, lane, p.a.args);
+                        for (int s = 0; s < 2; ++s) {
+                            uint32_t cuts;
+                            item[s].look(i + 1, lane, p.a.args, &takes[s], &cuts);
+                        }
                     }
                     // The step in the middle of a run of tiles that both streams take, without the general step's
                     // questions: this warp's instructions between two products are on every tile's path.
@@ -642,10 +646,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             bool any = false;
             uint32_t takes = 0, cuts = 0;
             for (int i = 0, count = it.last - it.first; i < count; ++i, takes >>= 1, cuts >>= 1) {
-                if ((i & 31) == 0) {
-                    takes = it.takes(i, lane, p.a.args);
-                    cuts = it.cuts(i, lane, p.a.args);
-                }
+                if ((i & 31) == 0) it.look(i, lane, p.a.args, &takes, &cuts);
                 at.advance();  // from the keys' slot to the values'
                 if (!(takes & 1u)) {
                     at.advance();

@@ -31,11 +31,6 @@ _DTYPES = {torch.float32: _native.DCN_DTYPE_F32, torch.float16: _native.DCN_DTYP
 _KINDS = {"rms": _native.DCN_NORM_RMS, "layer": _native.DCN_NORM_LAYER}
 
 
-def _heads(t) -> _native.DcnHeads:
-    token, head, _ = t.stride()
-    return _native.DcnHeads(t.data_ptr(), token, head)
-
-
 def _said(name, t, wanted) -> InvalidArgument:
     return InvalidArgument(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}; {wanted} is wanted")
 
@@ -64,10 +59,14 @@ class CudaTokenOps:
             raise InvalidArgument(f"element type {t.dtype}: float32, float16 or bfloat16 is wanted")
         return dtype
 
-    def _tokens(self, name, t, shape, dtype) -> None:
+    def _tokens(self, name, t, shape, dtype) -> _native.DcnHeads:
         """A [tokens][heads][head_dim] tensor with unit stride along head_dim on this device."""
-        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index or (t.stride(2) != 1 and shape[2] > 1):
-            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device} with unit stride along the last dimension")
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index:
+            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device}")
+        token, head, unit = t.stride()
+        if unit != 1 and shape[2] > 1:
+            raise _said(name, t, "unit stride along the last dimension")
+        return _native.DcnHeads(t.data_ptr(), token, head)
 
     def _whole(self, name, t, shape, dtype) -> int:
         """The address of a contiguous tensor of a given shape and type on this device."""
@@ -90,9 +89,9 @@ class CudaTokenOps:
     def _new(self, like, stream):
         """A contiguous tensor like another one, from the memory of the stream that will write it."""
         if stream is None:
-            return like.new_empty(like.shape)
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
         with torch.cuda.stream(stream):
-            return like.new_empty(like.shape)
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
 
     def _rotation(self, positions, frequencies, pairs, interleaved, tokens) -> _native.DcnRotation:
         if len(pairs) != 3 or min(pairs) < 0:
@@ -112,13 +111,16 @@ class CudaTokenOps:
         index = self._index
         if k_cache.get_device() != index or v_cache.get_device() != index or k_unit != 1 or v_unit != 1:
             raise InvalidArgument(f"k_cache and v_cache need unit stride along head_dim and to be on {self.device}")
-        if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != index or table.stride(1) != 1:
+        if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != index:
             raise _said("table", table, f"a [streams, columns] int32 tensor on {self.device}")
         pages, page_size, heads, head_dim = shape
         streams, columns = table.shape
+        table_stride, unit = table.stride()
+        if unit != 1 and columns > 1:
+            raise _said("table", table, "unit stride along its rows")
         return _native.DcnPagedCache(
             k_cache.data_ptr(), v_cache.data_ptr(), k_page, k_slot, k_head, v_page, v_slot, v_head, pages, page_size, heads,
-            head_dim, self._dtype(k_cache), streams, columns, 0, table.stride(0), table.data_ptr(),
+            head_dim, self._dtype(k_cache), streams, columns, 0, table_stride, table.data_ptr(),
             self._whole("starts", starts, (streams + 1,), torch.int32), self._whole("lengths", lengths, (streams,), torch.int32))
 
     # -- positions and cache -----------------------------------------------------
@@ -133,14 +135,12 @@ class CudaTokenOps:
             raise InvalidArgument(f"x is {tuple(x.shape)}; [tokens, heads, head_dim] is wanted")
         shape = x.shape
         tokens, heads, head_dim = shape
-        self._tokens("x", x, shape, x.dtype)
+        x_at = self._tokens("x", x, shape, x.dtype)
         rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
         if out is None:
             out = self._new(x, stream)
-        else:
-            self._tokens("out", out, shape, x.dtype)
-        self._call(stream, self.lib.dcn_token_rotary, self._dtype(x), tokens, heads, head_dim, rotation, _heads(x),
-                   _heads(out))
+        out_at = self._tokens("out", out, shape, x.dtype)
+        self._call(stream, self.lib.dcn_token_rotary, self._dtype(x), tokens, heads, head_dim, rotation, x_at, out_at)
         return out
 
     def append(self, k, v, k_cache, v_cache, table, starts, lengths, q=None, positions=None, frequencies=None,
@@ -157,27 +157,27 @@ class CudaTokenOps:
             raise InvalidArgument(f"k is {tuple(k.shape)}; [tokens, kv_heads, head_dim] is wanted")
         tokens, dtype = k.shape[0], k_cache.dtype
         _, _, heads, head_dim = k_cache.shape
-        self._tokens("k", k, (tokens, heads, head_dim), dtype)
-        self._tokens("v", v, (tokens, heads, head_dim), dtype)
+        k_at = self._tokens("k", k, (tokens, heads, head_dim), dtype)
+        v_at = self._tokens("v", v, (tokens, heads, head_dim), dtype)
         rotation = None
         if positions is not None:
             rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
         elif frequencies is not None or any(pairs):
             raise InvalidArgument("a rotation needs positions")
-        q_heads, q_from, q_to = 0, None, None
+        q_heads, q_at, q_out_at = 0, None, None
         if q is not None:
             if q.dim() != 3:
                 raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
             q_heads = q.shape[1]
-            self._tokens("q", q, (tokens, q_heads, head_dim), dtype)
+            q_shape = (tokens, q_heads, head_dim)
+            q_at = self._tokens("q", q, q_shape, dtype)
             if q_out is None:
                 q_out = self._new(q, stream)
-            else:
-                self._tokens("q_out", q_out, (tokens, q_heads, head_dim), dtype)
-            q_from, q_to = _heads(q), _heads(q_out)
+            q_out_at = self._tokens("q_out", q_out, q_shape, dtype)
         elif q_out is not None:
             raise InvalidArgument("q_out needs q")
-        self._call(stream, self.lib.dcn_token_append, cache, tokens, rotation, _heads(k), _heads(v), q_heads, q_from, q_to)
+        self._call(stream, self.lib.dcn_token_append, cache, tokens, rotation, k_at, v_at, q_heads, q_at,
+                   q_out_at)
         return q_out
 
     # -- attention ---------------------------------------------------------------
@@ -195,13 +195,12 @@ class CudaTokenOps:
         cache = self._cache(k_cache, v_cache, table, starts, lengths)
         shape = q.shape
         tokens, q_heads, head_dim = shape
-        self._tokens("q", q, (tokens, q_heads, k_cache.shape[3]), k_cache.dtype)
+        q_at = self._tokens("q", q, (tokens, q_heads, cache.head_dim), k_cache.dtype)
         args = _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame,
                                              1.0 / math.sqrt(head_dim) if scale is None else scale, 0)
-        if out is not None:
-            self._tokens("out", out, shape, q.dtype)
-        else:
+        if out is None:
             out = self._new(q, stream)
+        out_at = self._tokens("out", out, shape, q.dtype)
         need = self.lib.dcn_token_attention_workspace_bytes(cache, args)
         given, address = need, None
         if workspace is not None:
@@ -215,7 +214,7 @@ class CudaTokenOps:
                 with torch.cuda.stream(stream):
                     workspace = q.new_empty(need, dtype=torch.uint8)
             address = workspace.data_ptr()
-        self._call(stream, self.lib.dcn_token_attention, cache, args, _heads(q), _heads(out), address, given)
+        self._call(stream, self.lib.dcn_token_attention, cache, args, q_at, out_at, address, given)
         return out
 
     def attention_workspace_bytes(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0,
@@ -233,19 +232,24 @@ class CudaTokenOps:
         """Address and row stride of a [groups, width] tensor with unit stride along its rows."""
         if t is None:
             return None, 0
-        row, unit = t.stride() if t.dim() == 2 else (0, 0)
-        if t.shape[-1] != width or t.shape[0] < groups or t.dtype != dtype or t.get_device() != self._index or \
-                (unit != 1 and width > 1):
-            raise _said(name, t, f"[{groups}, {width}] {dtype} on {self.device} with unit stride along its rows")
+        shape = t.shape
+        if len(shape) != 2 or shape[1] != width or shape[0] < groups or t.dtype != dtype or t.get_device() != self._index:
+            raise _said(name, t, f"[{groups}, {width}] {dtype} on {self.device}")
+        row, unit = t.stride()
+        if unit != 1 and width > 1:
+            raise _said(name, t, "unit stride along its rows")
         return t.data_ptr(), row
 
     def _rows(self, name, t, shape, dtype):
         """Address and row stride of a [rows, width] tensor with unit stride along its rows."""
         if t is None:
             return None, 0
-        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index or (t.stride(1) != 1 and shape[1] > 1):
-            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device} with unit stride along its rows")
-        return t.data_ptr(), t.stride(0)
+        if t.shape != shape or t.dtype != dtype or t.get_device() != self._index:
+            raise _said(name, t, f"{tuple(shape)} {dtype} on {self.device}")
+        row, unit = t.stride()
+        if unit != 1 and shape[1] > 1:
+            raise _said(name, t, "unit stride along its rows")
+        return t.data_ptr(), row
 
     def _norm(self, x, residual, post, post_weight, post_bias, gate, residual_scale, kind, weight, bias, scale, shift, group,
               eps, hidden, out, stream):

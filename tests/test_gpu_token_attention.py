@@ -85,6 +85,9 @@ CASES = {
     "more_queries_than_keys": ([10, 0, 200], [25, 4, 200], 4, 2, 64, 16, 30, 1, 1),
     "streams_70": (list(range(1, 71)), [k % 3 for k in range(70)], 2, 2, 64, 16, 20, 2, 1),
     "two_tiles": ([256], [256], 1, 1, 128, 64, 1000, 0, 1),
+    # more row blocks than SMs, the last ones split: one and several tokens a stream, one stream without keys
+    "tokens_tail": ([300 + 37 * k for k in range(40)], [1] * 40, 8, 4, 64, 32, 900, 3, 1),
+    "tokens_tail_steps": ([0] + [1500 + 11 * k for k in range(54)], [2] + [1 + k % 5 for k in range(54)], 3, 3, 128, 64, 700, 0, 1),
     "four_tiles_long": ([3000], [600], 2, 1, 128, 64, 500, 100, 1),
 }
 
