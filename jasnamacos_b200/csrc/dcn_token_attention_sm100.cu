@@ -38,6 +38,7 @@ constexpr int kSoftmaxWarps = 8;    // two warpgroups
 constexpr int kThreads = 384;       // 2 softmax warpgroups, then 2 product warps, 2 load warps
 constexpr int kTmemCols = 512;      // S0, S1 (128 each), O0, O1 (head_dim each)
 constexpr uint32_t kTmemO = 256;
+constexpr uint32_t kTmemP = 384;    // P0, P1 of head_dim 64; of 128, where there is no room, P lies over S
 constexpr float kLag = 8.0f;        // log2 of how far the maximum in use may lag
 constexpr int kSmCount = 148;
 
@@ -47,6 +48,9 @@ struct Layout {
     static constexpr int kSlots = (Shared ? 5 : 3) * (D == 64 ? 2 : 1);  // tiles of a ring
     static constexpr int kTileBytes = kKeys * D * 2;
     static constexpr int kQTiles = Shared ? 2 : 1;
+    // P in columns of its own: the next tile's scores are made as soon as this tile's have been read, while
+    // their exponentials run, and no longer wait for the second product.
+    static constexpr bool kApart = D == 64;
 };
 
 struct KernelParams {
@@ -187,7 +191,7 @@ struct alignas(1024) Smem {
     uint8_t q[L::kQTiles][L::kTileBytes];
     uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
     uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
-    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], o_full[2], scanned[2], merge_ready, merge_read, drain;
+    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], s_read[2], pv_done[2], o_full[2], scanned[2], merge_ready, merge_read, drain;
     // The current item of each softmax warp and of the product warp's two streams, kept here: the 128
     // scores of a row need the registers.
     Item item[kSoftmaxWarps + 2];
@@ -351,6 +355,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             mbar_init(&sm.s_full[s], 1);
             mbar_init(&sm.p_full[s][0], 4);
             mbar_init(&sm.p_full[s][1], 4);
+            mbar_init(&sm.s_read[s], 4);
+            mbar_init(&sm.pv_done[s], 1);
             mbar_init(&sm.o_full[s], 1);
             mbar_init(&sm.scanned[s], 4);
             sm.dirty[s][0] = sm.dirty[s][1] = -1;
@@ -388,7 +394,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             constexpr uint32_t kIdescO = make_idesc_f16_f32(kRows, D) | kTypes | (1u << 16);  // B: N contiguous
             constexpr int kLastRing = L::kRings - 1;
             RingAt<L::kSlots> at[L::kRings];
-            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, read_phase[2] = {0, 0};
             const uint32_t issue = elect_one();
             uint64_t q_desc[2], k_desc[L::kRings], v_desc[L::kRings];
 #pragma unroll
@@ -413,12 +419,20 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     tc_fence_after();
 #pragma unroll
                     for (int k = h * kKeys / 2; k < (h + 1) * kKeys / 2; k += 16) {
-                        umma_f16_ts_if(issue, tmem + kTmemO + s * D, tmem + s * kKeys + k / 2, desc + (k * 128 >> 4), kIdescO,
-                                       more);
+                        umma_f16_ts_if(issue, tmem + kTmemO + s * D,
+                                       tmem + (L::kApart ? kTmemP + s * (kKeys / 2) : s * kKeys) + k / 2,
+                                       desc + (k * 128 >> 4), kIdescO, more);
                         more = 1;
                     }
                 }
                 p_phase[s] ^= 1u;
+                if (L::kApart) umma_commit_if(issue, &sm.pv_done[s]);
+                return true;
+            };
+            auto scores_read = [&](int s) {
+                if (!wait(&sm.s_read[s], read_phase[s])) return false;
+                read_phase[s] ^= 1u;
+                tc_fence_after();
                 return true;
             };
             auto scores = [&](int s, int r, int slot) {  // S = Q K^T
@@ -458,6 +472,19 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     // The step in the middle of a run of tiles that both streams take, without the general step's
                     // questions: this warp's instructions between two products are on every tile's path.
                     while (took[0] & took[1] & takes[0] & takes[1] & (((i + 1) & 31) != 31)) {
+                        if (L::kApart) {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) {
+                                const int r = s < kLastRing ? s : kLastRing;
+                                RingAt<L::kSlots> here = at[r];
+                                here.advance();
+                                if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
+                                if (!scores_read(s)) break;
+                                scores(s, r, here.slot);
+                                if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
+                            }
+                            if (!ok) break;
+                        }
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
                             const int r = s < kLastRing ? s : kLastRing;
@@ -466,10 +493,12 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             if (!second(s, r, here.slot, more[s])) break;
                             if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
-                            if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
-                            scores(s, r, here.slot);
+                            if (!L::kApart) {
+                                if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
+                                scores(s, r, here.slot);
+                                if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
+                            }
                             if (!Shared || s == 1) {
-                                umma_commit_if(issue, &sm.empty[r][here.slot]);
                                 here.advance();
                                 at[r] = here;
                             }
@@ -492,7 +521,10 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         }
                         if (i >= 0 && i < count[s]) {
                             if (!wait(&sm.full[r][here.slot], here.parity)) break;
-                            if (took[s] && !second(s, r, here.slot, more[s])) break;
+                            if (took[s]) {
+                                if (L::kApart && !scores_read(s)) break;
+                                if (!second(s, r, here.slot, more[s])) break;
+                            }
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
                         }
@@ -574,12 +606,13 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         const int ring = Shared ? 0 : s;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + lanes + s * kKeys, o_tmem = tmem + lanes + kTmemO + s * D;
+        const uint32_t p_tmem = L::kApart ? tmem + lanes + kTmemP + s * (kKeys / 2) : s_tmem;
         const int row_token = row * p.per_ratio >> 16, row_head = row - row_token * p.ratio;
         const bool row_used = row_token < p.tile_tokens;
         RingAt<L::kSlots> at;
         uint32_t s_phase = 0, item_phase = 0, free_phase = 0, merge_phase = 0;
         int item_number = 0;
-        bool ok = true, q_loaded = false;
+        bool ok = true, q_loaded = false, tiles_done = false;
         auto wait = [&](uint64_t *bar, uint32_t parity) {  // the whole warp gives up together
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
             if (!ok && lane == 0) give_up(sm, p.err);
@@ -687,6 +720,11 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     for (int k = 0; k < kKeys; k += 32) tmem_ld_32x32b_x32(s_tmem + k, x + k);
 #pragma unroll
                     for (int k = 0; k < kKeys; k += 32) tmem_wait_ld_x32(x + k);
+                    if (L::kApart) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.s_read[s]);
+                    }
                     if (cut) {
                         const int base = it.key_tile(it.first + i) * kKeys;
                         if (valid && !(base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high))) {
@@ -707,6 +745,12 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[kKeys - 4 + j]));
                     const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                    // The last tile's second product has ended: O may be scaled, P written again.  (Where P lies over S
+                    // this tile's scores were issued after it.)
+                    if (L::kApart && tiles_done) {
+                        if (!wait(&sm.pv_done[s], s_phase)) break;
+                        tc_fence_after();
+                    }
                     if (!any) {
                         m = t;
                     } else if (__any_sync(0xffffffffu, (t - m) * p.c > kLag)) {
@@ -737,18 +781,22 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             sum[k / 2 % 2] = add_pair(sum[k / 2 % 2], pair_of(a, b));
                             x[k / 2] = pack_pair<T>(a, b);
                         }
-                        tmem_st_32x32b_x32_wait(s_tmem + h * 32, x + h * 32);
+                        tmem_st_32x32b_x32_wait(p_tmem + h * 32, x + h * 32);
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sm.p_full[s][h]);
                     }
                     const uint64_t sums = add_pair(sum[0], sum[1]);
                     l += low_of(sums) + high_of(sums);
-                } else if (lane == 0) {
-                    mbar_arrive(&sm.p_full[s][0]);
-                    mbar_arrive(&sm.p_full[s][1]);
+                } else {  // no row of the step: keeps pace with the other warps, a phase at a time
+                    if (L::kApart && lane == 0) mbar_arrive(&sm.s_read[s]);
+                    if (L::kApart && tiles_done && !wait(&sm.pv_done[s], s_phase)) break;
+                    if (lane == 0) {
+                        mbar_arrive(&sm.p_full[s][0]);
+                        mbar_arrive(&sm.p_full[s][1]);
+                    }
                 }
-                any = true;
+                any = tiles_done = true;
             }
             if (!ok) break;
             if (!rows) continue;
