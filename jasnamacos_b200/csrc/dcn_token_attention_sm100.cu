@@ -104,7 +104,6 @@ struct Item {
     int both_last;                  // and the end of both streams' ranges
     int pinned_tiles, window_tile;  // the list: tiles [0, pinned_tiles), then from window_tile
     int part;
-    Span both;                      // of the rows of both streams
 
     __device__ __forceinline__ int key_tile(int i) const {
         return i < pinned_tiles ? i : window_tile + (i - pinned_tiles);
@@ -122,7 +121,7 @@ struct Item {
         const Span seen = span(a);
         const int base = key_tile(at) * kKeys;
         *takes = __ballot_sync(0xffffffffu, in && seen.tile_some(base));
-        *cuts = __ballot_sync(0xffffffffu, in && !seen.tile_all(base));
+        *cuts = __ballot_sync(0xffffffffu, in && seen.tile_some(base) && !seen.tile_all(base));
     }
     __device__ __forceinline__ Span span(const dcn_token_attention_args &a) const {
         Span out;
@@ -135,6 +134,7 @@ template <bool Shared>
 struct Walk {
     int w, block;  // item, and its row block (-1: take the item's first)
     int s;         // stream of tiles
+    Span both;     // of the rows of both of the block's streams
 
     __device__ __forceinline__ explicit Walk(int stream_of_tiles) : w(blockIdx.x), block(-1), s(stream_of_tiles) {}
     __device__ __forceinline__ bool next(const KernelParams &p, Item &it) {
@@ -168,10 +168,10 @@ struct Walk {
             int tiles = 0;
             it.pinned_tiles = it.window_tile = 0;
             if (it.length > 0 && it.position(end - 1) >= 0) {
-                it.both.set(max(it.position(t0), 0), it.position(end - 1), it.length, p.a.args);
-                it.pinned_tiles = (min(it.both.pinned, it.both.high) + kKeys - 1) / kKeys;
-                it.window_tile = max(it.both.low / kKeys, it.pinned_tiles);
-                tiles = it.pinned_tiles + max(0, (it.both.high + kKeys - 1) / kKeys - it.window_tile);
+                both.set(max(it.position(t0), 0), it.position(end - 1), it.length, p.a.args);
+                it.pinned_tiles = (min(both.pinned, both.high) + kKeys - 1) / kKeys;
+                it.window_tile = max(both.low / kKeys, it.pinned_tiles);
+                tiles = it.pinned_tiles + max(0, (both.high + kKeys - 1) / kKeys - it.window_tile);
             }
             const uint32_t parts = Shared ? splits : 2 * splits;
             const int each = (static_cast<uint32_t>(tiles) + parts - 1) / parts;
@@ -191,12 +191,13 @@ struct alignas(1024) Smem {
     uint8_t q[L::kQTiles][L::kTileBytes];
     uint8_t kv[L::kRings][L::kSlots][L::kTileBytes];
     uint64_t full[L::kRings][L::kSlots], empty[L::kRings][L::kSlots];
-    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], s_read[2], pv_done[2], o_full[2], scanned[2], merge_ready, merge_read, drain;
+    uint64_t q_full[2], q_free, s_full[2], p_full[2][2], s_read[2], pv_done[2], o_full[2], scan_go, scanned, merge_ready, merge_read, drain;
     // The current item of each softmax warp and of the product warp's two streams, kept here: the 128
     // scores of a row need the registers.
     Item item[kSoftmaxWarps + 2];
     float2 other_ml[kRows];  // stream 1's (c m, l), where stream 0 merges the two
-    int dirty[2][2];
+    int other_dirty;         // and whether its rows are to be done alone
+    int dirty[2][2];         // by the parity of an item's number: the last item whose rows are to be done alone
     int abort_flag;
     uint32_t tmem_base;
 };
@@ -218,6 +219,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The lowest n bits of a word; none for n <= 0, all for n >= 32.
+__device__ __forceinline__ uint32_t bits_below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
 // Two FP32 values in one register pair, and the instructions that take two at a time.
@@ -257,10 +263,33 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Bit 15 or 31 is set where the lower or upper value of a pair is not finite: one more in the exponent's
+// last place carries out of an exponent of ones, and of no other.
 template <typename T>
-__device__ __forceinline__ bool pair_not_finite(uint32_t w) {
-    constexpr uint32_t kExponent = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-    return (w & kExponent) == kExponent || ((w >> 16) & kExponent) == kExponent;
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+    constexpr uint32_t kExponents = __is_same(T, __half) ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kOnes = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+    return (pair & kExponents) + kOnes;
+}
+
+// Looks through one key's row of a tile of values for what is not finite.  Where it finds something and no
+// row of the block sees the key (hidden), the row becomes zeros; true where some row does.
+template <typename T, int D>
+__device__ __forceinline__ bool scan_values(uint8_t *tile, int row, bool hidden) {
+    uint8_t *v_row = tile + row * 128;
+    auto pack_at = [&](int e) {
+        return reinterpret_cast<uint4 *>(v_row + (e / 8) * (kKeys * 128) + (((e % 8) ^ (row % 8)) * 16));
+    };
+    uint32_t found = 0;
+#pragma unroll 8
+    for (int e = 0; e < D / 8; ++e) {
+        const uint4 v = *pack_at(e);
+        found |= not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w);
+    }
+    if ((found & 0x80008000u) == 0) return false;
+    if (!hidden) return true;
+    for (int e = 0; e < D / 8; ++e) *pack_at(e) = make_uint4(0, 0, 0, 0);
+    return false;
 }
 
 // One of the failure path's records: some wait ran out.
@@ -339,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map) {
     using L = Layout<D, Shared>;
+    static_assert(sizeof(Smem<D, Shared>) + 1024 <= 227 * 1024, "a block's shared memory");
     extern __shared__ uint8_t raw[];
     Smem<D, Shared> &sm = *reinterpret_cast<Smem<D, Shared> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
     volatile int *abort_flag = &sm.abort_flag;
@@ -350,6 +380,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 mbar_init(&sm.full[r][i], 1);
                 mbar_init(&sm.empty[r][i], 1);
             }
+        mbar_init(&sm.scan_go, 1);
+        mbar_init(&sm.scanned, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.q_full[s], kRows);
             mbar_init(&sm.s_full[s], 1);
@@ -357,8 +389,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             mbar_init(&sm.p_full[s][1], 4);
             mbar_init(&sm.s_read[s], 4);
             mbar_init(&sm.pv_done[s], 1);
-            mbar_init(&sm.o_full[s], 1);
-            mbar_init(&sm.scanned[s], 4);
+            mbar_init(&sm.o_full[s], 2);
             sm.dirty[s][0] = sm.dirty[s][1] = -1;
         }
         mbar_init(&sm.q_free, 1);
@@ -394,6 +425,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             constexpr uint32_t kIdescO = make_idesc_f16_f32(kRows, D) | kTypes | (1u << 16);  // B: N contiguous
             constexpr int kLastRing = L::kRings - 1;
             RingAt<L::kSlots> at[L::kRings];
+            uint32_t scan_phase = 0;
             uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, read_phase[2] = {0, 0};
             const uint32_t issue = elect_one();
             uint64_t q_desc[2], k_desc[L::kRings], v_desc[L::kRings];
@@ -410,6 +442,13 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
                 if (!ok && lane == 0) give_up(sm, p.err);
                 return ok;
+            };
+            // Shared: tiles of values that some row does not see all of are looked through before their
+            // product, by a warp of its own: asked for with the tile's scores, waited for before its product.
+            auto scanned = [&]() {
+                if (!wait(&sm.scanned, scan_phase)) return false;
+                scan_phase ^= 1u;
+                return true;
             };
             auto second = [&](int s, int r, int slot, uint32_t &more) {  // O += P V, half a tile's keys at a time
                 const uint64_t desc = v_desc[r] + static_cast<uint32_t>(slot * (L::kTileBytes >> 4));
@@ -460,18 +499,20 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 const int count[2] = {item[0].last - item[0].first, item[1].last - item[1].first};
                 const int steps = max(count[0], count[1]);
                 uint32_t more[2] = {0, 0}, takes[2] = {0, 0}, took[2] = {0, 0};
+                uint32_t cuts = 0, scan = 0;  // Shared: tiles to be looked through, and whether the last is one
                 // Step i: the second product of tile i, then the scores of tile i + 1.
                 for (int i = -1; ok && i < steps; ++i) {
                     if (((i + 1) & 31) == 0) {  // bit j: whether a stream takes tile i + 1 + j of its list
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
-                            uint32_t cuts;
-                            item[s].look(i + 1, lane, p.a.args, &takes[s], &cuts);
+                            uint32_t cut;
+                            item[s].look(i + 1, lane, p.a.args, &takes[s], &cut);
+                            cuts = Shared ? s == 0 ? cut : cuts | cut : 0;
                         }
                     }
                     // The step in the middle of a run of tiles that both streams take, without the general step's
                     // questions: this warp's instructions between two products are on every tile's path.
-                    while (took[0] & took[1] & takes[0] & takes[1] & (((i + 1) & 31) != 31)) {
+                    while (took[0] & took[1] & takes[0] & takes[1] & ~(scan | cuts) & (((i + 1) & 31) != 31)) {
                         if (L::kApart) {
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
@@ -507,6 +548,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         ++i;
                         takes[0] >>= 1;
                         takes[1] >>= 1;
+                        cuts >>= 1;
                     }
                     if (!ok) break;
 #pragma unroll
@@ -515,12 +557,13 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         const bool release = !Shared || s == 1;  // the last to read the tile
                         const bool take = takes[s] & 1u;
                         RingAt<L::kSlots> here = at[r];
-                        if (i < 0 && item[s].rows() && (Shared || s == 0)) {
+                        if (i < 0 && item[s].rows()) {
                             if (!wait(&sm.q_full[s], q_phase[s])) break;
                             q_phase[s] ^= 1u;
                         }
                         if (i >= 0 && i < count[s]) {
                             if (!wait(&sm.full[r][here.slot], here.parity)) break;
+                            if (scan && s == 0 && !scanned()) break;
                             if (took[s]) {
                                 if (L::kApart && !scores_read(s)) break;
                                 if (!second(s, r, here.slot, more[s])) break;
@@ -534,25 +577,83 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                                 tc_fence_after();
                                 scores(s, r, here.slot);
                             }
+                            if ((cuts & 1u) && s == 0 && lane == 0) mbar_arrive(&sm.scan_go);
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
                         }
                         if (i + 1 == count[s] && item[s].rows()) {
                             // Once an item, with or without products: the softmax warpgroup moves on only after
                             // it, so no barrier of the item runs a phase ahead of this warp.
+                            // The second arrival passes on what was written where values were looked through.
                             umma_commit_if(issue, &sm.o_full[s]);
+                            if (lane == 0) mbar_arrive(&sm.o_full[s]);
                             if (!Shared && s == 1) umma_commit_if(issue, &sm.q_free);
                         }
                         took[s] = take;
                         takes[s] >>= 1;
                         if (release) at[r] = here;
                     }
+                    scan = cuts & 1u;
+                    cuts >>= 1;
                 }
             }
             // Every product issued has ended before the block lets go of its memory.
             umma_commit_if(issue, &sm.drain);
             mbar_wait_bounded(&sm.drain, 0, nullptr);
             __syncwarp();
+        } else if (Shared && warp == kSoftmaxWarps + 1) {
+            // ------------------------------------------------------------------------ scan
+            // A row's weights are 0 for the keys that it does not see, and 0 x non-finite is not 0.  So in each
+            // tile of values that some row does not see all of, a key that no row of the block sees becomes
+            // zeros, and where a key that only some see is not finite, those rows' tile is marked, and its rows
+            // are done alone at the end.  (With one row tile a block, where memory is the bound, the softmax
+            // warps do it while they wait for the scores.)
+            RingAt<L::kSlots> at;
+            uint32_t go_phase = 0;
+            int number = 0;  // items with tiles so far
+            bool ok = true;
+            Walk<Shared> walk0(0), walk1(1);
+            while (ok) {
+                Item item0, item1;
+                if (!walk0.next(p, item0) || !walk1.next(p, item1)) break;
+                const Span span0 = item0.span(p.a.args), span1 = item1.span(p.a.args);
+                const int count = item0.last - item0.first;
+                uint32_t takes, cuts0 = 0, cuts1 = 0;
+                for (int i = 0; ok && i < count; ++i, cuts0 >>= 1, cuts1 >>= 1) {
+                    if ((i & 31) == 0) {
+                        item0.look(i, lane, p.a.args, &takes, &cuts0);
+                        item1.look(i, lane, p.a.args, &takes, &cuts1);
+                    }
+                    at.advance();  // from the keys' slot to the values'
+                    const bool cut0 = cuts0 & 1u, cut1 = cuts1 & 1u;
+                    if (cut0 || cut1) {
+                        // The slot's earlier tiles have been used when this one is asked for, and it stays until it
+                        // has been looked through: its barrier's next phase is this tile's.
+                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.scan_go, go_phase, abort_flag) &&
+                                                         mbar_wait_bounded(&sm.full[0][at.slot], at.parity, abort_flag));
+                        if (!ok) {
+                            if (lane == 0) give_up(sm, p.err);
+                            break;
+                        }
+                        go_phase ^= 1u;
+                        const int base = item0.key_tile(item0.first + i) * kKeys;
+                        for (int row = lane; row < kKeys; row += 32) {
+                            const int key = base + row;
+                            const bool some0 = cut0 && !span0.all(key), some1 = cut1 && !span1.all(key);
+                            if (!some0 && !some1) continue;
+                            if (scan_values<T, D>(sm.kv[0][at.slot], row, !walk0.both.some(key))) {
+                                if (some0) *static_cast<volatile int *>(&sm.dirty[0][number & 1]) = number;
+                                if (some1) *static_cast<volatile int *>(&sm.dirty[1][number & 1]) = number;
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.scanned);
+                    }
+                    at.advance();
+                }
+                number += count > 0;
+            }
         } else if (warp >= kSoftmaxWarps + 2 && warp < kSoftmaxWarps + 2 + L::kRings) {
             const int s = warp - (kSoftmaxWarps + 2);
             // -------------------------------------------------------------------- loads of ring s
@@ -603,15 +704,14 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         // ---------------------------------------------------------------------- softmax of stream s
         const int s = warp >> 2;
         const int row = threadIdx.x & (kRows - 1);
-        const int ring = Shared ? 0 : s;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + lanes + s * kKeys, o_tmem = tmem + lanes + kTmemO + s * D;
         const uint32_t p_tmem = L::kApart ? tmem + lanes + kTmemP + s * (kKeys / 2) : s_tmem;
         const int row_token = row * p.per_ratio >> 16, row_head = row - row_token * p.ratio;
         const bool row_used = row_token < p.tile_tokens;
-        RingAt<L::kSlots> at;
         uint32_t s_phase = 0, item_phase = 0, free_phase = 0, merge_phase = 0;
-        int item_number = 0;
+        int tile_items = 0;  // items with tiles so far
+        RingAt<L::kSlots> at;
         bool ok = true, q_loaded = false, tiles_done = false;
         auto wait = [&](uint64_t *bar, uint32_t parity) {  // the whole warp gives up together
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
@@ -620,7 +720,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         };
         Walk<Shared> walk(s);
         const Item &it = sm.item[warp];
-        for (;; ++item_number) {
+        for (;;) {
             {
                 Item next;
                 if (!ok || !walk.next(p, next)) break;
@@ -666,6 +766,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&sm.q_full[s]);
+            } else if (rows) {
+                mbar_arrive(&sm.q_full[s]);  // stream 0 loads the tile; this stream is ready for the item
             }
             int seen_first, seen_low, seen_high;
             {
@@ -680,37 +782,25 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             uint32_t takes = 0, cuts = 0;
             for (int i = 0, count = it.last - it.first; i < count; ++i, takes >>= 1, cuts >>= 1) {
                 if ((i & 31) == 0) it.look(i, lane, p.a.args, &takes, &cuts);
-                at.advance();  // from the keys' slot to the values'
+                if (!Shared) at.advance();  // from the keys' slot to the values'
                 if (!(takes & 1u)) {
-                    at.advance();
+                    if (!Shared) at.advance();
                     continue;
                 }
                 const bool cut = cuts & 1u;
-                if (cut) {
-                    const Span span = it.span(p.a.args);
-                    const int base = it.key_tile(it.first + i) * kKeys;
-                    // Some rows' weights are 0 for some keys here, and 0 x non-finite is not 0.  A key that
-                    // no row of the block sees becomes zeros; where only some see it, all rows are done alone.
-                    if (!wait(&sm.full[ring][at.slot], at.parity)) break;
-                    const int key = base + row;
-                    if (!span.all(key)) {
-                        uint8_t *v_row = sm.kv[ring][at.slot] + row * 128;
-                        const bool hidden = !it.both.some(key);
-#pragma unroll
-                        for (int e = 0; e < D / 8; ++e) {
-                            uint4 *at16 = reinterpret_cast<uint4 *>(v_row + (e / 8) * (kKeys * 128) + (((e % 8) ^ (row % 8)) * 16));
-                            const uint4 v = *at16;
-                            if (pair_not_finite<T>(v.x) || pair_not_finite<T>(v.y) || pair_not_finite<T>(v.z) ||
-                                pair_not_finite<T>(v.w)) {
-                                if (hidden) *at16 = make_uint4(0, 0, 0, 0);
-                                else *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) = item_number;
-                            }
-                        }
+                if (!Shared) {
+                    if (cut) {
+                        if (!wait(&sm.full[s][at.slot], at.parity)) break;
+                        const Span span = it.span(p.a.args);
+                        const int key = it.key_tile(it.first + i) * kKeys + row;
+                        // (Both streams have the same rows.)
+                        if (!span.all(key) && scan_values<T, D>(sm.kv[s][at.slot], row, !span.some(key)))
+                            *static_cast<volatile int *>(&sm.dirty[s][tile_items & 1]) = tile_items;
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
+                    at.advance();
                 }
-                at.advance();
                 if (!wait(&sm.s_full[s], s_phase)) break;
                 s_phase ^= 1u;
                 if (warp_used) {
@@ -728,10 +818,15 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     if (cut) {
                         const int base = it.key_tile(it.first + i) * kKeys;
                         if (valid && !(base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high))) {
-                            const int a = seen_first - base, lo = seen_low - base, hi = seen_high - base;
 #pragma unroll
-                            for (int k = 0; k < kKeys; ++k)
-                                if (!(k < a || (k >= lo && k < hi))) x[k] = 0xff800000u;  // -inf
+                            for (int w = 0; w < kKeys; w += 32) {
+                                // Bit k: key base + w + k is seen.
+                                const uint32_t mask = bits_below(seen_first - base - w) |
+                                                      (bits_below(seen_high - base - w) & ~bits_below(seen_low - base - w));
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    if (!(mask >> k & 1u)) x[w + k] = 0xff800000u;  // -inf
+                            }
                         }
                         __syncwarp();
                     }
@@ -799,13 +894,14 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 any = tiles_done = true;
             }
             if (!ok) break;
+            const bool has_tiles = it.last > it.first;
+            const int tile_item = tile_items;  // this item's number among those with tiles, as the scan counts them
+            tile_items += has_tiles;
             if (!rows) continue;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.scanned[s]);
-            if (!wait(&sm.o_full[s], item_phase) || !wait(&sm.scanned[s], item_phase)) break;
+            if (!wait(&sm.o_full[s], item_phase)) break;
             item_phase ^= 1u;
             tc_fence_after();
-            bool alone = *reinterpret_cast<volatile int *>(&sm.dirty[s][item_number & 1]) == item_number;
+            bool alone = has_tiles && *reinterpret_cast<volatile int *>(&sm.dirty[s][tile_item & 1]) == tile_item;
             const int64_t at_row = static_cast<int64_t>(it.start + token) * p.a.args.q_heads + head;
             const int64_t part_row = static_cast<int64_t>(it.part) * p.a.args.tokens * p.a.args.q_heads + at_row;
             T *out = static_cast<T *>(p.a.out.data) + (it.start + token) * p.a.out.token_stride + head * p.a.out.head_stride;
@@ -816,6 +912,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             float mc = m * p.c;
             if (merge && s == 1) {
                 sm.other_ml[row] = any ? make_float2(mc, l) : other;
+                if (row == 0) sm.other_dirty = alone;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.merge_ready);
                 if (!wait(&sm.merge_read, merge_phase)) break;  // its O may be written again
@@ -827,7 +924,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 merge_phase ^= 1u;
                 tc_fence_after();
                 other = sm.other_ml[row];
-                alone |= *reinterpret_cast<volatile int *>(&sm.dirty[1][item_number & 1]) == item_number;
+                alone |= sm.other_dirty != 0;
             }
             if (alone) {
                 if (valid) {
