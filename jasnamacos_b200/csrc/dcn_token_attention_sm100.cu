@@ -512,7 +512,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     }
                     // The step in the middle of a run of tiles that both streams take, without the general step's
                     // questions: this warp's instructions between two products are on every tile's path.
-                    while (took[0] & took[1] & takes[0] & takes[1] & ~(scan | cuts) & (((i + 1) & 31) != 31)) {
+                    while (took[0] & took[1] & takes[0] & takes[1] & (((i + 1) & 31) != 31)) {
+                        if (scan && !scanned()) break;
                         if (L::kApart) {
 #pragma unroll
                             for (int s = 0; s < 2; ++s) {
@@ -522,6 +523,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                                 if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
                                 if (!scores_read(s)) break;
                                 scores(s, r, here.slot);
+                                if ((cuts & 1u) && s == 0 && lane == 0) mbar_arrive(&sm.scan_go);
                                 if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             }
                             if (!ok) break;
@@ -537,6 +539,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             if (!L::kApart) {
                                 if ((!Shared || s == 0) && !wait(&sm.full[r][here.slot], here.parity)) break;
                                 scores(s, r, here.slot);
+                                if ((cuts & 1u) && s == 0 && lane == 0) mbar_arrive(&sm.scan_go);
                                 if (!Shared || s == 1) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             }
                             if (!Shared || s == 1) {
@@ -548,6 +551,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         ++i;
                         takes[0] >>= 1;
                         takes[1] >>= 1;
+                        scan = cuts & 1u;
                         cuts >>= 1;
                     }
                     if (!ok) break;
