@@ -231,7 +231,7 @@ def test_attention_bounds_are_only_hints(ops):
     """Smaller and larger max_q and max_kv than the streams have: the same result to its bound."""
     s = make(10, [2000, 600], [300, 20], 4, 2, 64, 64, F16)
     want, bound = ref.attention(**s, window=700, sinks=2)
-    for max_q, max_kv in ((300, 2000), (1000, 100000), (300, 0), (300, 10)):
+    for max_q, max_kv in ((300, 2000), (1000, 100000), (300, 0), (300, 10), (1, 2000), (0, 0), (20, 600)):
         ref.check(ops.attention(**s, max_q=max_q, max_kv=max_kv, window=700, sinks=2), want, bound)
 
 
