@@ -809,6 +809,25 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 s_phase ^= 1u;
                 if (warp_used) {
                     tc_fence_after();
+                    if (cut) {
+                        // Hidden keys' scores become -inf where they lie, 32 columns at a time, which keeps the
+                        // selects out of the code that every tile runs through.
+                        const int base = it.key_tile(it.first + i) * kKeys;
+                        // Bit k: key base + w + k is seen; rows of no query keep theirs.
+                        const int first = valid ? seen_first - base : kKeys, low = seen_low - base, high = seen_high - base;
+#pragma unroll 1
+                        for (int w = 0; w < kKeys; w += 32) {
+                            const uint32_t mask = bits_below(first - w) | (bits_below(high - w) & ~bits_below(low - w));
+                            if (__all_sync(0xffffffffu, mask == 0xffffffffu)) continue;
+                            uint32_t y[32];
+                            tmem_ld_32x32b_x32(s_tmem + w, y);
+                            tmem_wait_ld_x32(y);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (!(mask >> k & 1u)) y[k] = 0xff800000u;
+                            tmem_st_32x32b_x32_wait(s_tmem + w, y);
+                        }
+                    }
                     uint32_t x[kKeys];
 #pragma unroll
                     for (int k = 0; k < kKeys; k += 32) tmem_ld_32x32b_x32(s_tmem + k, x + k);
@@ -818,21 +837,6 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sm.s_read[s]);
-                    }
-                    if (cut) {
-                        const int base = it.key_tile(it.first + i) * kKeys;
-                        if (valid && !(base + kKeys <= seen_first || (base >= seen_low && base + kKeys <= seen_high))) {
-#pragma unroll
-                            for (int w = 0; w < kKeys; w += 32) {
-                                // Bit k: key base + w + k is seen.
-                                const uint32_t mask = bits_below(seen_first - base - w) |
-                                                      (bits_below(seen_high - base - w) & ~bits_below(seen_low - base - w));
-#pragma unroll
-                                for (int k = 0; k < 32; ++k)
-                                    if (!(mask >> k & 1u)) x[w + k] = 0xff800000u;  // -inf
-                            }
-                        }
-                        __syncwarp();
                     }
                     float top[4];
 #pragma unroll
