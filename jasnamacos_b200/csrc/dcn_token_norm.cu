@@ -167,16 +167,16 @@ __global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const __grid_con
 // which costs it no registers.
 enum { kGate = 0, kScale, kShift, kPostWeight, kPostBias };
 
-constexpr int kFoldedWarps = 8;
 constexpr int kFoldedRows = 64;  // rows a block, at least
 constexpr int kStages = 2;       // rows of a warp in shared memory
+constexpr int kFoldedBytes = 112 * 1024;  // shared memory of a block: two an SM
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(32 * kFoldedWarps) token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a,
+template <typename T, int NV, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps) token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a,
                                                                              int block_rows, uint32_t *err) {
     constexpr int VEC = kVec<T>;
     extern __shared__ float4 raw[];
-    __shared__ uint64_t landed[kFoldedWarps][kStages];
+    __shared__ uint64_t landed[kWarps][kStages];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int width = a.width, bytes = width * static_cast<int>(sizeof(T));
     const int coefficients = a.post ? 5 : 3, tensors = a.residual ? 2 : 1;
@@ -197,13 +197,17 @@ __global__ void __launch_bounds__(32 * kFoldedWarps) token_norm_folded_kernel(co
         for (int s = 0; s < kStages; ++s) mbar_init(&landed[warp][s], 1);
         fence_mbarrier_init();
         for (int s = 0; s < kStages; ++s)
-            if (row + s * kFoldedWarps < end) fetch(row + s * kFoldedWarps, s);
+            if (row + s * kWarps < end) fetch(row + s * kWarps, s);
     }
     __syncwarp();
+    // Where element c of a folded vector lies.  A lane reads eight in a row as two float4: the first four of
+    // every eight come before all the others, or the reads of a warp, 32 bytes apart, would meet in half
+    // of the banks.
+    auto place = [&](int c) { return VEC == 8 ? (c & 4) * (width / 8) + (c >> 3) * 4 + (c & 3) : c; };
     auto coefficient = [&](int which, int c, float (&v)[VEC]) {
 #pragma unroll
         for (int j = 0; j < VEC; j += 4)
-            *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(folded + which * width + c + j);
+            *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(folded + which * width + place(c + j));
     };
     bool ok = true;
     float *scratch = nullptr;  // a row is one warp's
@@ -213,21 +217,21 @@ __global__ void __launch_bounds__(32 * kFoldedWarps) token_norm_folded_kernel(co
         const int64_t g = segment / a.group;
         const int64_t segment_end = min((g + 1) * a.group, end);
         __syncthreads();
-        for (int c = threadIdx.x; c < width; c += 32 * kFoldedWarps) {
+        for (int c = threadIdx.x; c < width; c += 32 * kWarps) {
             auto one = [&](const void *base, int64_t offset, float otherwise) {
                 return base ? to_float<T>(*at(base, offset + c)) : otherwise;
             };
             const float scale = 1.0f + one(a.scale, g * a.scale_stride, 0.0f);
-            folded[kGate * width + c] = one(a.gate, g * a.gate_stride, 1.0f);
-            folded[kScale * width + c] = one(a.weight, 0, 1.0f) * scale;
-            folded[kShift * width + c] = one(a.bias, 0, 0.0f) * scale + one(a.shift, g * a.shift_stride, 0.0f);
+            folded[kGate * width + place(c)] = one(a.gate, g * a.gate_stride, 1.0f);
+            folded[kScale * width + place(c)] = one(a.weight, 0, 1.0f) * scale;
+            folded[kShift * width + place(c)] = one(a.bias, 0, 0.0f) * scale + one(a.shift, g * a.shift_stride, 0.0f);
             if (a.post) {
-                folded[kPostWeight * width + c] = one(a.post_weight, 0, 1.0f);
-                folded[kPostBias * width + c] = one(a.post_bias, 0, 0.0f);
+                folded[kPostWeight * width + place(c)] = one(a.post_weight, 0, 1.0f);
+                folded[kPostBias * width + place(c)] = one(a.post_bias, 0, 0.0f);
             }
         }
         __syncthreads();
-        for (; row < segment_end; row += kFoldedWarps) {
+        for (; row < segment_end; row += kWarps) {
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&landed[warp][stage], parity, nullptr));
             if (!ok) {
                 if (lane == 0) atomicOr(err, kErrWaitTimeout);
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(32 * kFoldedWarps) token_norm_folded_kernel(co
                 }
             }
             __syncwarp();
-            if (lane == 0 && row + kStages * kFoldedWarps < end) fetch(row + kStages * kFoldedWarps, stage);
+            if (lane == 0 && row + kStages * kWarps < end) fetch(row + kStages * kWarps, stage);
             if (++stage == kStages) {
                 stage = 0;
                 parity ^= 1u;
@@ -307,36 +311,50 @@ cudaError_t launch(const dcn_token_norm_args &a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-// Shared memory of the folded kernel.
-size_t folded_bytes(const dcn_token_norm_args &a, size_t element) {
-    return (a.post ? 5 : 3) * sizeof(float) * a.width + kFoldedWarps * kStages * (a.residual ? 2 : 1) * element * a.width;
+// Shared memory of a block of the folded kernel.
+size_t folded_bytes(const dcn_token_norm_args &a, size_t element, int warps) {
+    return (a.post ? 5 : 3) * sizeof(float) * a.width + warps * kStages * (a.residual ? 2 : 1) * element * a.width;
 }
 
-template <typename T, int NV>
+template <typename T, int NV, int kWarps>
 cudaError_t launch_folded(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
-    // Even shares of the rows for the blocks that are on the GPU at once (three an SM by registers, fewer
-    // by shared memory), so that no round of blocks is left half empty.
-    const size_t smem = folded_bytes(a, sizeof(T));
-    const int64_t per_sm = static_cast<int64_t>(220 * 1024 / (smem + 1024));
-    const int64_t at_once = 148 * (per_sm < 3 ? per_sm : 3);
+    // Even shares of the rows for the blocks that are on the GPU at once, so that no round of blocks is left
+    // half empty (24 warps an SM by registers, fewer by shared memory).
+    const size_t smem = folded_bytes(a, sizeof(T), kWarps);
+    const int64_t fit = static_cast<int64_t>(226 * 1024 / (smem + 1024)), most = 24 / kWarps;
+    const int64_t at_once = 148 * (fit < most ? fit : most);
     const int64_t rounds = (a.rows + at_once * 256 - 1) / (at_once * 256);
     int64_t rows = (a.rows + at_once * rounds - 1) / (at_once * rounds);
     if (rows < kFoldedRows) rows = kFoldedRows;
-    token_norm_folded_kernel<T, NV><<<static_cast<unsigned>((a.rows + rows - 1) / rows), 32 * kFoldedWarps, smem, stream>>>(
+    token_norm_folded_kernel<T, NV, kWarps><<<static_cast<unsigned>((a.rows + rows - 1) / rows), 32 * kWarps, smem, stream>>>(
         a, static_cast<int>(rows), err);
     return cudaGetLastError();
 }
 
+// Blocks of 12 warps where two fit an SM, else of 6: 61,440 rows of 1,024 FP16 elements with a residual (505 MB)
+// take 89.5 us in blocks of 12 and 97 in blocks of 8; with a post norm's vectors 12 leave room for one block.
+template <typename T, int NV>
+cudaError_t launch_folded(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
+    return folded_bytes(a, sizeof(T), 12) <= kFoldedBytes ? launch_folded<T, NV, 12>(a, err, stream)
+                                                         : launch_folded<T, NV, 6>(a, err, stream);
+}
+
+template <typename T, int NV>
+cudaError_t prepare_folded() {
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(token_norm_folded_kernel<T, NV, 12>),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kFoldedBytes);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(reinterpret_cast<const void *>(token_norm_folded_kernel<T, NV, 6>),
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kFoldedBytes);
+    return e;
+}
+
 template <typename T>
 cudaError_t prepare() {
-    const void *kernels[] = {reinterpret_cast<const void *>(token_norm_folded_kernel<T, 1>),
-                             reinterpret_cast<const void *>(token_norm_folded_kernel<T, 2>),
-                             reinterpret_cast<const void *>(token_norm_folded_kernel<T, 4>)};
-    for (const void *fn : kernels) {
-        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 * 1024);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    cudaError_t e = prepare_folded<T, 1>();
+    if (e == cudaSuccess) e = prepare_folded<T, 2>();
+    if (e == cudaSuccess) e = prepare_folded<T, 4>();
+    return e;
 }
 
 // Whether every row and vector may be read in 16-byte packs.
