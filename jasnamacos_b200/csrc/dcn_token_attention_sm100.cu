@@ -37,7 +37,6 @@
 #include <mutex>
 
 #include "dcn_token_attention.cuh"
-#include "dcn_tokens.cuh"
 
 namespace dcn {
 namespace {
@@ -309,68 +308,36 @@ __device__ __forceinline__ void give_up(S &s, uint32_t *err) {
     *reinterpret_cast<volatile int *>(&s.abort_flag) = 1;
 }
 
-// out of one row, alone, from its visible keys in key tiles [first, last) of the item's list: for
-// rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in the
-// product would reach the others).  Slow and rare.
+// The rows of a warp (row_of: this lane's, or none), one after another, from their visible keys in the item's
+// key tiles: for rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in
+// the product would reach the others).  Slow and rare.
 template <typename T, int D>
-__device__ __noinline__ void row_alone(const KernelParams &p, const Item it, int token, int head, const Visible seen, T *out,
-                                       float *part_o, float2 *part_ml) {
-    const dcn_paged_cache &c = p.a.cache;
-    const T *q = static_cast<const T *>(p.a.q.data) + (it.start + token) * p.a.q.token_stride + head * p.a.q.head_stride;
-    const float sign = p.negate ? -1.0f : 1.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int e0 = -32; e0 < D; e0 += 32) {  // first the maximum and sum, then 32 elements a pass
-        float acc[32];
+__device__ __noinline__ void rows_alone(const KernelParams &p, const Item it, bool valid, int token, int head,
+                                        const Visible seen, int64_t part_row) {
+    const int lane = threadIdx.x & 31;
+    // The range of the list of tiles, as keys.
+    const int64_t begin[2] = {static_cast<int64_t>(it.first) * kKeys,
+                              (it.window_tile + max(it.first - it.pinned_tiles, 0)) * static_cast<int64_t>(kKeys)};
+    const int64_t end[2] = {static_cast<int64_t>(min(it.last, it.pinned_tiles)) * kKeys,
+                            it.last > it.pinned_tiles ? (it.window_tile + it.last - it.pinned_tiles) * static_cast<int64_t>(kKeys) : 0};
+    for (uint32_t left = __ballot_sync(0xffffffffu, valid); left != 0; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        const int row_token = __shfl_sync(0xffffffffu, token, from), row_head = __shfl_sync(0xffffffffu, head, from);
+        const Visible row_seen{__shfl_sync(0xffffffffu, seen.first, from), __shfl_sync(0xffffffffu, seen.low, from),
+                               __shfl_sync(0xffffffffu, seen.high, from)};
+        const int64_t row_part = __shfl_sync(0xffffffffu, part_row, from);
+        const T *q = static_cast<const T *>(p.a.q.data) + (it.start + row_token) * p.a.q.token_stride + row_head * p.a.q.head_stride;
+        RowByWarp<T, D / 32> row;
+        row.run(p.a.cache, it.stream, it.kv_head, q, p.negate ? -p.c : p.c, row_seen, begin, end);
+        const bool none = row_seen.first <= 0 && row_seen.high <= row_seen.low;
+        T *out = static_cast<T *>(p.a.out.data) + (it.start + row_token) * p.a.out.token_stride + row_head * p.a.out.head_stride;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-        for (int i = it.first; i < it.last; ++i) {
-            for (int key = it.key_tile(i) * kKeys; key < (it.key_tile(i) + 1) * kKeys; ++key) {
-                if (!(key < seen.first || (key >= seen.low && key < seen.high))) continue;
-                const int column = key / c.page_size;
-                const int page = column < c.table_columns ? c.table[it.stream * c.table_stride + column] : -1;
-                const bool has = page >= 0 && page < c.pages;
-                const int64_t slot = key - column * c.page_size;
-                float score = 0.0f;
-                if (has) {
-                    const T *k = static_cast<const T *>(c.keys) + page * c.key_page_stride + slot * c.key_slot_stride +
-                                 it.kv_head * c.key_head_stride;
-#pragma unroll 4
-                    for (int e = 0; e < D; e += 8) {
-                        float qv[8], kv[8];
-                        unpack<T, 8>(load_pack<T, 8>(q + e), qv);
-                        unpack<T, 8>(load_pack<T, 8>(k + e), kv);
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) score = fmaf(qv[n] * sign, kv[n], score);
-                    }
-                }
-                score *= p.c;
-                if (e0 < 0) {
-                    const float top = fmaxf(m, score);
-                    const float base = top == -INFINITY ? 0.0f : top;
-                    l = l * exp2_approx(m - base) + exp2_approx(score - base);
-                    m = top;
-                } else if (has) {
-                    const T *v = static_cast<const T *>(c.values) + page * c.value_page_stride +
-                                 slot * c.value_slot_stride + it.kv_head * c.value_head_stride + e0;
-                    const float w = exp2_approx(score - (m == -INFINITY ? 0.0f : m));
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        float vv[8];
-                        unpack<T, 8>(load_pack<T, 8>(v + e), vv);
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) acc[e + n] = fmaf(w, vv[n], acc[e + n]);
-                    }
-                }
-            }
+        for (int i = 0; i < D / 32; ++i) {
+            if (p.part_o) p.part_o[row_part * D + i * 32 + lane] = row.acc[i];
+            else out[i * 32 + lane] = from_float<T>(none ? 0.0f : row.acc[i] / row.l);
         }
-        if (e0 < 0) continue;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            if (part_o) part_o[e0 + e] = acc[e];
-            else out[e0 + e] = from_float<T>(seen.first <= 0 && seen.high <= seen.low ? 0.0f : acc[e] / l);
-        }
+        if (p.part_o && lane == 0) p.part_ml[row_part] = make_float2(row.m, row.l);
     }
-    if (part_o) *part_ml = make_float2(m, l);
 }
 
 template <typename T, int D, bool Shared>
@@ -947,12 +914,9 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                 alone |= sm.other_dirty != 0;
             }
             if (alone) {
-                if (valid) {
-                    Item all = it;
-                    if (merge) all.last = it.both_last;
-                    row_alone<T, D>(p, all, token, head, Visible{seen_first, seen_low, seen_high}, out,
-                                    p.part_o ? p.part_o + part_row * D : nullptr, p.part_ml ? p.part_ml + part_row : nullptr);
-                }
+                Item all = it;
+                if (merge) all.last = it.both_last;
+                rows_alone<T, D>(p, all, valid, token, head, Visible{seen_first, seen_low, seen_high}, part_row);
                 __syncwarp();
             } else if (warp_used) {
                 const bool none = seen_first <= 0 && seen_high <= seen_low;
