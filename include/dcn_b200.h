@@ -506,8 +506,9 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
  * hidden keys and values hold, non-finite values included, does not reach the result.
  * q_heads is a multiple of the cache's heads: query head h reads key head h / (q_heads / heads).
  *   max_q    at least the longest step starts[b + 1] - starts[b]
- *   max_kv   at least the largest length (it sizes the split over keys; a longer stream is
- *            still computed in full)
+ *   max_kv   at least the largest length
+ * Both only size the launch and its split over keys: longer steps and streams are still computed in
+ * full.  Rows of out at or past starts[streams], tokens of no stream, are left as they are.
  * FP16 and BF16 with head_dim 64 or 128, 16-byte aligned tensors and strides, page_size a multiple
  * of 8 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
  * 256, other strides) on CUDA cores.  `workspace` holds

@@ -66,7 +66,7 @@ dcn_status check_attention(const dcn_paged_cache *c, const dcn_token_attention_a
     dcn_status st = check_cache(c);
     if (st != DCN_OK) return st;
     if (a == nullptr || a->reserved != 0) return DCN_ERR_INVALID_ARGUMENT;
-    if (a->tokens < 0 || a->q_heads <= 0 || a->q_heads > kMaxHeads || a->q_heads % c->heads != 0 ||
+    if (a->tokens < 0 || a->tokens >= (int64_t{1} << 31) || a->q_heads <= 0 || a->q_heads > kMaxHeads || a->q_heads % c->heads != 0 ||
         a->tokens * a->q_heads >= (int64_t{1} << 31) || a->max_q < 0 || a->max_kv < 0)
         return DCN_ERR_INVALID_SHAPE;
     if (a->window < 1 || a->sinks < 0 || a->frame < 1 || !(a->scale == a->scale)) return DCN_ERR_INVALID_ARGUMENT;

@@ -50,6 +50,7 @@ constexpr uint32_t kTmemO = 256;
 constexpr uint32_t kTmemP = 384;    // P0, P1 of head_dim 64; of 128, where there is no room, P lies over S
 constexpr float kLag = 8.0f;        // log2 of how far the maximum in use may lag
 constexpr int kSmCount = 148;
+constexpr int64_t kMaxItems = int64_t{1} << 20;  // of a launch, where one stream's row blocks are what makes them many
 
 template <int D, bool Shared>
 struct Layout {
@@ -1078,16 +1079,23 @@ Plan make_plan(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
     Plan plan{};
     plan.ratio = a.q_heads / c.heads;
     plan.tile_tokens = kRows / plan.ratio;
-    plan.shared = a.max_q > plan.tile_tokens;
+    // The limits are hints and may be loose: no step is longer than all tokens, no stream than its row of pages.
+    const int32_t max_q = static_cast<int32_t>(a.max_q < a.tokens ? a.max_q : a.tokens);
+    const int64_t room = static_cast<int64_t>(c.table_columns) * c.page_size;
+    const int32_t max_kv = static_cast<int32_t>(a.max_kv < room ? a.max_kv : room);
+    plan.shared = max_q > plan.tile_tokens;
     const int block_tokens = plan.tile_tokens * (plan.shared ? 2 : 1);
-    plan.row_blocks = a.max_q > 0 ? (a.max_q - 1) / block_tokens + 1 : 1;
+    plan.row_blocks = max_q > 0 ? (max_q - 1) / block_tokens + 1 : 1;
+    // One long step among many streams: an item takes several row blocks (Walk) rather than have millions of empty items.
+    const int64_t most = kMaxItems / (static_cast<int64_t>(c.heads) * c.streams + 1) + 1;
+    if (plan.row_blocks > most) plan.row_blocks = static_cast<int>(most);
     const int64_t blocks = static_cast<int64_t>(plan.row_blocks) * c.heads * c.streams;
     // Key tiles of a row block, at most.
     auto keys_of = [&](int32_t frames) {
-        return frames > a.max_kv / a.frame ? int64_t{a.max_kv} : static_cast<int64_t>(frames) * a.frame;
+        return frames > max_kv / a.frame ? int64_t{max_kv} : static_cast<int64_t>(frames) * a.frame;
     };
     const int64_t span = keys_of(a.window) + keys_of(a.sinks) + block_tokens;
-    const int64_t tiles = (span < a.max_kv ? span : a.max_kv) / kKeys + 1;
+    const int64_t tiles = (span < max_kv ? span : max_kv) / kKeys + 1;
     // Split the keys of a row block over as many blocks as make the whole shortest: rounds of the
     // GPU's blocks, each as long as its tiles plus a fixed part (start, queries, result), plus the join.
     const int streams = plan.shared ? 1 : 2;

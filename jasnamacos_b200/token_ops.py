@@ -181,6 +181,13 @@ class CudaTokenOps:
         return q_out
 
     # -- attention ---------------------------------------------------------------
+    def _attention_args(self, tokens, q_heads, max_q, max_kv, window, sinks, frame, scale):
+        # ctypes keeps an integer's low bits only.
+        if max(max_q, max_kv, window, sinks, frame) >= 1 << 31 or min(max_q, max_kv, window, sinks, frame) < 0:
+            raise InvalidArgument(f"max_q {max_q}, max_kv {max_kv}, window {window}, sinks {sinks}, frame {frame}: "
+                                  "32-bit counts are wanted")
+        return _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame, scale, 0)
+
     def attention(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0, frame=1, scale=None,
                   out=None, workspace=None, stream=None):
         """Attention of a step's queries `q` [tokens, q_heads, head_dim] over the cache of :meth:`append`.
@@ -188,16 +195,16 @@ class CudaTokenOps:
         A frame is `frame` consecutive positions.  A query sees its own frame and those before it in the
         stream, of these the last `window` frames and the first `sinks` frames; frame = 1 is plain causal
         attention with a sliding window and first tokens that stay.  `max_q` bounds the streams' steps and
-        `max_kv` their lengths.  `scale` defaults to head_dim ** -0.5.  A query that sees no key gives zeros.
-        `workspace` (uint8, :meth:`attention_workspace_bytes`) is taken from PyTorch when not given."""
+        `max_kv` their lengths.  `scale` defaults to head_dim ** -0.5.  A query that sees no key gives zeros;
+        rows of tokens that belong to no stream are not written (nor cleared in a new `out`).  `workspace` (uint8, :meth:`attention_workspace_bytes`) is taken from PyTorch when not given."""
         if q.dim() != 3:
             raise InvalidArgument(f"q is {tuple(q.shape)}; [tokens, q_heads, head_dim] is wanted")
         cache = self._cache(k_cache, v_cache, table, starts, lengths)
         shape = q.shape
         tokens, q_heads, head_dim = shape
         q_at = self._tokens("q", q, (tokens, q_heads, cache.head_dim), k_cache.dtype)
-        args = _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame,
-                                             1.0 / math.sqrt(head_dim) if scale is None else scale, 0)
+        args = self._attention_args(tokens, q_heads, max_q, max_kv, window, sinks, frame,
+                                    1.0 / math.sqrt(head_dim) if scale is None else scale)
         if out is None:
             out = self._new(q, stream)
         out_at = self._tokens("out", out, shape, q.dtype)
@@ -221,7 +228,7 @@ class CudaTokenOps:
                                   frame=1) -> int:
         """Bytes of scratch that :meth:`attention` takes for these tensors."""
         cache = self._cache(k_cache, v_cache, table, starts, lengths)
-        args = _native.DcnTokenAttentionArgs(q.shape[0], q.shape[1], max_q, max_kv, window, sinks, frame, 1.0, 0)
+        args = self._attention_args(q.shape[0], q.shape[1], max_q, max_kv, window, sinks, frame, 1.0)
         return int(self.lib.dcn_token_attention_workspace_bytes(cache, args))
 
     # -- norms -------------------------------------------------------------------

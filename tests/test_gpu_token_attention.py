@@ -272,3 +272,19 @@ def test_attention_refused(ops):
     if need:
         with pytest.raises(InvalidArgument):
             ops.attention(**good, workspace=torch.empty(need - 16, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("lengths,steps", [([2000, 600], [300, 20]), ([700] * 40, [1] * 40), ([900] + [50] * 200, [600] + [1] * 200)])
+def test_attention_without_known_limits(ops, lengths, steps):
+    """The largest max_q, max_kv and window there are: the launch follows the tensors."""
+    s = make(13, lengths, steps, 4, 2, 64, 64, F16)
+    want, bound = ref.attention(**s, window=5000)
+    most = 2**31 - 1
+    ref.check(ops.attention(**s, max_q=most, max_kv=most, window=most), want, bound)
+
+
+@pytest.mark.parametrize("name", ["max_q", "max_kv", "window", "sinks", "frame"])
+def test_attention_counts_past_32_bits_are_refused(ops, name):
+    s = make(14, [100], [10], 4, 2, 64, 16, F16)
+    with pytest.raises(InvalidArgument):
+        ops.attention(**(dict(s, max_q=10, max_kv=100, window=4) | {name: 2**32 + 4}))

@@ -162,3 +162,21 @@ def test_attention_tensor_refusals(lib):
 ])
 def test_norm_refusals(lib, changes, want):
     assert lib.dcn_token_norm(norm_args(**changes), None) == want
+
+
+@pytest.mark.parametrize("tokens", [1 << 31, 1 << 61, (1 << 63) - 1])
+def test_attention_token_counts_past_32_bits(lib, tokens):
+    """Refused as such: tokens * q_heads does not wrap to something small."""
+    args = attention_args(tokens=tokens, q_heads=8)
+    assert lib.dcn_token_attention_workspace_bytes(cache(), args) == 0
+    assert lib.dcn_token_attention(cache(), args, heads(), heads(), None, 0, None) == SHAPE
+
+
+@pytest.mark.parametrize("q_heads", [2, 8])
+def test_attention_workspace_with_loose_limits(lib, q_heads):
+    """max_q and max_kv far past the tokens and the table cost no more scratch than the tight ones."""
+    wide = cache(table_columns=1024, table_stride=1024)
+    tight = lib.dcn_token_attention_workspace_bytes(wide, attention_args(q_heads=q_heads, max_q=8, max_kv=16384, window=1 << 30))
+    loose = lib.dcn_token_attention_workspace_bytes(
+        wide, attention_args(q_heads=q_heads, max_q=2**31 - 1, max_kv=2**31 - 1, window=1 << 30))
+    assert 0 < tight == loose
