@@ -33,7 +33,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_direct_kernel(const Att
     const Visible seen = visible_keys(length - p.cache.starts[b + 1] + token, length, p.args.window, p.args.sinks,
                                       p.args.frame);
     RowByWarp<T, kMaxHeadDim / 32> row_sum;
-    row_sum.run(p.cache, b, kv_head, query[warp], p.args.scale * 1.4426950408889634f, seen, {0, seen.low}, {seen.first, seen.high});
+    row_sum.run(p.cache, b, kv_head, query[warp], p.args.scale * 1.4426950408889634f, seen, {0, seen.low}, {seen.first, seen.high},
+                nullptr);
     const bool none = seen.first <= 0 && seen.high <= seen.low;
     T *out = static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride;
 #pragma unroll

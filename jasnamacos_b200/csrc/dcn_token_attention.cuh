@@ -41,14 +41,15 @@ __host__ __device__ inline Visible visible_keys(int64_t position, int64_t length
 // One row: acc = sum_s exp2(c q.k_s - m) v_s and l = sum_s exp2(c q.k_s - m) over the keys of `parts` ranges
 // that the row sees, m the largest c q.k_s.  A whole warp's call: 32 keys at a time, one a lane for the products,
 // then the lanes hold the value's elements (lane + 32 i).  Hidden keys are never read, so what they hold
-// cannot matter.  `q` is read by every lane (one address at a time).
+// cannot matter.  `q` is read by every lane (one address at a time).  `beat` (nullable) counts on while it works,
+// for waits that would take a long row for a dead one.
 template <typename T, int kElements>
 struct RowByWarp {
     float acc[kElements], m, l;
 
     template <typename Q>
     __device__ __forceinline__ void run(const dcn_paged_cache &cache, int stream, int kv_head, const Q *q, float c,
-                                        const Visible &seen, const int64_t (&begin)[2], const int64_t (&end)[2]) {
+                                        const Visible &seen, const int64_t (&begin)[2], const int64_t (&end)[2], int *beat) {
         const int lane = threadIdx.x & 31, d = cache.head_dim;
         const T *keys = static_cast<const T *>(cache.keys) + kv_head * cache.key_head_stride;
         const T *values = static_cast<const T *>(cache.values) + kv_head * cache.value_head_stride;
@@ -58,6 +59,7 @@ struct RowByWarp {
         for (int i = 0; i < kElements; ++i) acc[i] = 0.0f;
         for (int part = 0; part < 2; ++part) {
             for (int64_t base = begin[part]; base < end[part]; base += 32) {
+                if (beat != nullptr && lane == 0) atomicAdd(beat, 1);
                 const int64_t key = base + lane;
                 float score = -INFINITY;
                 int64_t value_at = -1;

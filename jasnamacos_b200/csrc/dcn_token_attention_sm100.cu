@@ -209,6 +209,7 @@ struct alignas(1024) Smem {
     int other_dirty;         // and whether its rows are to be done alone
     int dirty[2][2];         // by the parity of an item's number: the last item whose rows are to be done alone
     int abort_flag;
+    int beat;                // counts on while rows are done alone, which may take longer than a wait's limit
     uint32_t tmem_base;
 };
 
@@ -309,12 +310,22 @@ __device__ __forceinline__ void give_up(S &s, uint32_t *err) {
     *reinterpret_cast<volatile int *>(&s.abort_flag) = 1;
 }
 
-// The rows of a warp (row_of: this lane's, or none), one after another, from their visible keys in the item's
-// key tiles: for rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in
+// A wait of bounded length, begun again for as long as some warp gets on with rows alone (whose work is finite).
+template <typename S>
+__device__ __forceinline__ bool wait_bounded(S &s, uint64_t *bar, uint32_t parity) {
+    while (true) {
+        const int beat = *reinterpret_cast<volatile int *>(&s.beat);
+        if (mbar_wait_bounded(bar, parity, &s.abort_flag)) return true;
+        if (*reinterpret_cast<volatile int *>(&s.abort_flag) || *reinterpret_cast<volatile int *>(&s.beat) == beat) return false;
+    }
+}
+
+// The rows of a warp (token and head: this lane's, where valid), one after another, from their visible keys in the
+// item's key tiles: for rows of a tile that holds a non-finite value which only some of its rows see (0 x inf in
 // the product would reach the others).  Slow and rare.
 template <typename T, int D>
 __device__ __noinline__ void rows_alone(const KernelParams &p, const Item it, bool valid, int token, int head,
-                                        const Visible seen, int64_t part_row) {
+                                        const Visible seen, int64_t part_row, int *beat) {
     const int lane = threadIdx.x & 31;
     // The range of the list of tiles, as keys.
     const int64_t begin[2] = {static_cast<int64_t>(it.first) * kKeys,
@@ -329,7 +340,7 @@ __device__ __noinline__ void rows_alone(const KernelParams &p, const Item it, bo
         const int64_t row_part = __shfl_sync(0xffffffffu, part_row, from);
         const T *q = static_cast<const T *>(p.a.q.data) + (it.start + row_token) * p.a.q.token_stride + row_head * p.a.q.head_stride;
         RowByWarp<T, D / 32> row;
-        row.run(p.a.cache, it.stream, it.kv_head, q, p.negate ? -p.c : p.c, row_seen, begin, end);
+        row.run(p.a.cache, it.stream, it.kv_head, q, p.negate ? -p.c : p.c, row_seen, begin, end, beat);
         const bool none = row_seen.first <= 0 && row_seen.high <= row_seen.low;
         T *out = static_cast<T *>(p.a.out.data) + (it.start + row_token) * p.a.out.token_stride + row_head * p.a.out.head_stride;
 #pragma unroll
@@ -349,7 +360,6 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
     static_assert(sizeof(Smem<D, Shared>) + 1024 <= 227 * 1024, "a block's shared memory");
     extern __shared__ uint8_t raw[];
     Smem<D, Shared> &sm = *reinterpret_cast<Smem<D, Shared> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
-    volatile int *abort_flag = &sm.abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -375,6 +385,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         mbar_init(&sm.merge_ready, 4);
         mbar_init(&sm.merge_read, 4);
         sm.abort_flag = 0;
+        sm.beat = 0;
         fence_mbarrier_init();
         prefetch_tensor_map(&k_map);
         prefetch_tensor_map(&v_map);
@@ -419,7 +430,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             bool ok = true;
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+                ok = __all_sync(0xffffffffu, wait_bounded(sm, bar, parity));
                 if (!ok && lane == 0) give_up(sm, p.err);
                 return ok;
             };
@@ -613,8 +624,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     if (cut0 || cut1) {
                         // The slot's earlier tiles have been used when this one is asked for, and it stays until it
                         // has been looked through: its barrier's next phase is this tile's.
-                        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.scan_go, go_phase, abort_flag) &&
-                                                         mbar_wait_bounded(&sm.full[0][at.slot], at.parity, abort_flag));
+                        ok = __all_sync(0xffffffffu, wait_bounded(sm, &sm.scan_go, go_phase) &&
+                                                         wait_bounded(sm, &sm.full[0][at.slot], at.parity));
                         if (!ok) {
                             if (lane == 0) give_up(sm, p.err);
                             break;
@@ -661,7 +672,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                     const int slot = key - column * p.a.cache.page_size;
 #pragma unroll 1
                     for (int v = 0; v < 2; ++v) {
-                        ok = mbar_wait_bounded(&sm.empty[s][at.slot], at.parity ^ 1u, abort_flag);
+                        ok = wait_bounded(sm, &sm.empty[s][at.slot], at.parity ^ 1u);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) {
                             if (lane == 0) give_up(sm, p.err);
@@ -698,7 +709,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
         RingAt<L::kSlots> at;
         bool ok = true, q_loaded = false, tiles_done = false;
         auto wait = [&](uint64_t *bar, uint32_t parity) {  // the whole warp gives up together
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+            ok = __all_sync(0xffffffffu, wait_bounded(sm, bar, parity));
             if (!ok && lane == 0) give_up(sm, p.err);
             return ok;
         };
@@ -917,7 +928,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             if (alone) {
                 Item all = it;
                 if (merge) all.last = it.both_last;
-                rows_alone<T, D>(p, all, valid, token, head, Visible{seen_first, seen_low, seen_high}, part_row);
+                rows_alone<T, D>(p, all, valid, token, head, Visible{seen_first, seen_low, seen_high}, part_row, &sm.beat);
                 __syncwarp();
             } else if (warp_used) {
                 const bool none = seen_first <= 0 && seen_high <= seen_low;

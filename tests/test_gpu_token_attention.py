@@ -288,3 +288,19 @@ def test_attention_counts_past_32_bits_are_refused(ops, name):
     s = make(14, [100], [10], 4, 2, 64, 16, F16)
     with pytest.raises(InvalidArgument):
         ops.attention(**(dict(s, max_q=10, max_kv=100, window=4) | {name: 2**32 + 4}))
+
+
+@pytest.mark.parametrize("length,step,at", [(131000, 300, 130900), (262143, 4, 262141)])
+def test_attention_long_rows_beside_non_finite_values(ops, length, step, at):
+    """A value that only a step's last rows see, over a long cache: its rows are done one by one, no wait runs
+    out meanwhile, and the rows before it are the formula's."""
+    s = make(15, [length], [step], 2, 1, 64, 64, F16)
+    want, bound = ref.attention(**s, window=10**6)
+    v = s["v_cache"].clone()
+    v[s["table"][0, at // 64].long(), at % 64, 0, 3] = float("inf")
+    out = run(ops, dict(s, v_cache=v), window=10**6)
+    torch.cuda.synchronize()
+    device_ok(ops)
+    clean = torch.arange(length - step, length, device="cuda") < at
+    ref.check(out[clean], want[clean], bound[clean])
+    assert not bool(torch.isfinite(out[~clean][..., 3]).any())
