@@ -167,13 +167,19 @@ __global__ void __launch_bounds__(NT *kTeams) token_norm_kernel(const __grid_con
 // which costs it no registers.
 enum { kGate = 0, kScale, kShift, kPostWeight, kPostBias };
 
-constexpr int kFoldedRows = 64;  // rows a block, at least
+// Where folding pays: a group's rows are worth its fold, and the whole is long enough to hide the blocks' start.
+// With a residual, FP16, folded and not (us): 61,440 rows of 1,024 in groups of 8 rows 148 and 154 (without a
+// residual 101 and 90), of 16 118 and 148, of 256 86 and 141; rows of 256 in groups of 32 31 and 30, of 64 27 and
+// 30.  Groups of 256: 4,096 rows of 1,024 11.4 and 17.1, of 512 6.9 and 6.4; 9,472 of 512 9.7 and 12.5.
+constexpr int64_t kFoldedPacks = 512 * 1024;  // 16-byte packs of a tensor
+constexpr int64_t kFoldedGroupPacks = 2048;   // and of a group
 constexpr int kStages = 2;       // rows of a warp in shared memory
 constexpr int kFoldedBytes = 112 * 1024;  // shared memory of a block: two an SM
 
+// (Registers for two blocks of 12 warps an SM; blocks of 6 leave room for more by themselves.)
 template <typename T, int NV, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps) token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a,
-                                                                             int block_rows, uint32_t *err) {
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 12 ? 2 : 0)
+token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a, int block_rows, uint32_t *err) {
     constexpr int VEC = kVec<T>;
     extern __shared__ float4 raw[];
     __shared__ uint64_t landed[kWarps][kStages];
@@ -318,21 +324,23 @@ size_t folded_bytes(const dcn_token_norm_args &a, size_t element, int warps) {
 
 template <typename T, int NV, int kWarps>
 cudaError_t launch_folded(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
-    // Even shares of the rows for the blocks that are on the GPU at once, so that no round of blocks is left
-    // half empty (24 warps an SM by registers, fewer by shared memory).
+    // Even shares of the rows for the blocks that are on the GPU at once, two an SM, so that no round of blocks is left
+    // half empty.  Long blocks pay their start once; of short ones, one folds while others stream.  61,440 rows of
+    // 1,024 (us): with a residual 93.6 in one round of blocks, 90.0 in two, 85.6 in four; without 48.7, 48.6, 50.6;
+    // with a post norm (blocks of 6 warps) 85.6, 95, 102.  Of 256, with a residual, 25.4 in one and 29.0 in four.
+    const int64_t packs = kWarps != 12 ? 32768 : a.residual ? 8192 : 16384;  // a block
+    const int64_t most = packs / (a.width / kVec<T>);
     const size_t smem = folded_bytes(a, sizeof(T), kWarps);
-    const int64_t fit = static_cast<int64_t>(226 * 1024 / (smem + 1024)), most = 24 / kWarps;
-    const int64_t at_once = 148 * (fit < most ? fit : most);
-    const int64_t rounds = (a.rows + at_once * 256 - 1) / (at_once * 256);
-    int64_t rows = (a.rows + at_once * rounds - 1) / (at_once * rounds);
-    if (rows < kFoldedRows) rows = kFoldedRows;
+    const int64_t at_once = 148 * 2;
+    const int64_t rounds = (a.rows + at_once * most - 1) / (at_once * most);
+    const int64_t rows = (a.rows + at_once * rounds - 1) / (at_once * rounds);
     token_norm_folded_kernel<T, NV, kWarps><<<static_cast<unsigned>((a.rows + rows - 1) / rows), 32 * kWarps, smem, stream>>>(
         a, static_cast<int>(rows), err);
     return cudaGetLastError();
 }
 
-// Blocks of 12 warps where two fit an SM, else of 6: 61,440 rows of 1,024 FP16 elements with a residual (505 MB)
-// take 89.5 us in blocks of 12 and 97 in blocks of 8; with a post norm's vectors 12 leave room for one block.
+// Blocks of 12 warps where two fit an SM (blocks of 8 took 8 % longer for 61,440 rows of 1,024 FP16 elements with a
+// residual), else of 6: with a post norm's vectors 12 leave room for one block.
 template <typename T, int NV>
 cudaError_t launch_folded(const dcn_token_norm_args &a, uint32_t *err, cudaStream_t stream) {
     return folded_bytes(a, sizeof(T), 12) <= kFoldedBytes ? launch_folded<T, NV, 12>(a, err, stream)
@@ -378,8 +386,7 @@ cudaError_t launch_typed(const dcn_token_norm_args &a, uint32_t *err, cudaStream
     constexpr int V = kVec<T>;
     if (vectorised<T>(a)) {
         const int packs = a.width / V;
-        // Folding pays where a block's rows are mostly of one group and every SM has some blocks.
-        if (packs <= 128 && a.group >= kFoldedRows / 2 && a.rows >= kFoldedRows * 296) {
+        if (packs <= 128 && a.group >= kFoldedGroupPacks / packs && a.rows * packs >= kFoldedPacks) {
             if (packs <= 32) return launch_folded<T, 1>(a, err, stream);
             if (packs <= 64) return launch_folded<T, 2>(a, err, stream);
             return launch_folded<T, 4>(a, err, stream);

@@ -343,3 +343,24 @@ def test_append_refused_and_other_stream(ops):
     out = ops.append(**good, q=k, stream=side)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, k) and torch.equal(k_cache, want_k) and torch.equal(v_cache, want_v)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,width,group,post", [(4101, 1024, 16, False), (4101, 1024, 17, True), (20011, 256, 130, True),
+                                                   (50003, 96, 400, False), (8200, 520, 100000, False), (9001, 1024, 5, False)])
+def test_residual_norm_by_rows_and_groups(ops, dtype, rows, width, group, post):
+    """On both sides of the sizes from which a block folds its groups' vectors; its share of rows is no multiple
+    of its warps, and ends inside a group."""
+    g = generator(rows + group)
+    groups = -(-rows // group)
+    x, residual = normal(g, (rows, width), dtype, 2.0) - 0.5, normal(g, (rows, width), dtype, 3.0)
+    shift, scale, gate = normal(g, (groups, 3, width), dtype, 0.4).unbind(1)
+    args = dict(gate=gate, kind="layer", weight=1 + normal(g, (width,), dtype, 0.1), scale=scale, shift=shift, group=group)
+    if post:
+        args |= dict(post_weight=1 + normal(g, (width,), dtype, 0.1), post_bias=normal(g, (width,), dtype, 0.1))
+    hidden, out = ops.residual_norm(x, residual, **args)
+    want_hidden, want_out = ref.norm(x, residual, **args)
+    ref.check(hidden, *want_hidden)
+    ref.check(out, *want_out)
+    plain = dict(scale=scale, shift=shift, group=group)
+    ref.check(ops.norm(x, **plain), *ref.norm(x, **plain)[1])
