@@ -1108,7 +1108,9 @@ Plan make_plan(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
     const int64_t span = keys_of(a.window) + keys_of(a.sinks) + block_tokens;
     const int64_t tiles = (span < max_kv ? span : max_kv) / kKeys + 1;
     // Split the keys of a row block over as many blocks as make the whole shortest: rounds of the
-    // GPU's blocks, each as long as its tiles plus a fixed part (start, queries, result), plus the join.
+    // GPU's blocks, each as long as its tiles plus a fixed part (start, queries, result), plus the join.  Both parts are
+    // three tiles' time: with a join for nothing, 1,944 tokens of 2 heads over 29 of their keys were split and took 25.0 us
+    // where unsplit they take 20.8; with one of a tile, or a start of one, 15 drawn calls stayed within 4 %.
     const int streams = plan.shared ? 1 : 2;
     int64_t best = INT64_MAX;
     plan.splits = 1;

@@ -268,7 +268,7 @@ class CudaTokenOps:
             raise InvalidArgument(f"kind {kind!r}: 'rms' or 'layer' is wanted")
         if group is None:
             group = max(1, rows)
-        if group < 1:
+        if not 1 <= group < 1 << 63:
             raise InvalidArgument(f"group {group}: at least one row shares a modulation row")
         groups = -(-rows // group)
         x_at, x_stride = self._rows("x", x, shape, dtype)

@@ -364,3 +364,10 @@ def test_residual_norm_by_rows_and_groups(ops, dtype, rows, width, group, post):
     ref.check(out, *want_out)
     plain = dict(scale=scale, shift=shift, group=group)
     ref.check(ops.norm(x, **plain), *ref.norm(x, **plain)[1])
+
+
+@pytest.mark.parametrize("group", [0, -1, 2**63, 2**64 + 1])
+def test_norm_group_out_of_range(ops, group):
+    """Refused, not cut to its low bits."""
+    with pytest.raises(InvalidArgument):
+        ops.norm(torch.zeros(2, 64, dtype=F16, device="cuda"), group=group)
