@@ -463,7 +463,8 @@ typedef struct dcn_rotation {
  *                  page_size = capacity)
  *   table          [streams][table_columns] page ids (row stride table_stride): position p of
  *                  stream b lies in page table[b][p / page_size], slot p % page_size
- *   starts         [streams + 1]: stream b's tokens of this step are [starts[b], starts[b + 1])
+ *   starts         [streams + 1], from 0 up and not falling: stream b's tokens of this step are [starts[b], starts[b + 1]);
+ *                  tokens before starts[0] are no stream's
  *   lengths        [streams]: tokens of stream b (below 2^31 - 1024), this step's included, so the i-th of its n
  *                  tokens of this step is at position lengths[b] - n + i
  * table, starts and lengths are read on the device.  Positions outside the table and page ids
@@ -492,8 +493,8 @@ dcn_status dcn_token_rotary(dcn_dtype dtype, int64_t tokens, int32_t heads, int3
 /* Appends a step's keys and values to the cache, and rotates its queries in the same launch: keys
  * are rotated and stored at their stream's positions, values are stored as they are, queries
  * (nullable: q_heads 0 and q, q_out NULL) are rotated into q_out (which may be q).  rotation NULL
- * stores keys as they are.  `tokens` is the token tensors' extent; tokens at or past
- * starts[streams] and tokens at a negative position are not stored. */
+ * stores keys as they are.  `tokens` is the token tensors' extent; tokens before starts[0],
+ * at or past starts[streams] and tokens at a negative position are not stored. */
 dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const dcn_rotation *rotation,
                             const dcn_heads *keys, const dcn_heads *values, int32_t q_heads,
                             const dcn_heads *q, const dcn_heads *q_out, dcn_stream stream);
@@ -508,7 +509,8 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
  *   max_q    at least the longest step starts[b + 1] - starts[b]
  *   max_kv   at least the largest length
  * Both only size the launch and its split over keys: longer steps and streams are still computed in
- * full.  Rows of out at or past starts[streams], tokens of no stream, are left as they are.
+ * full.  Rows of out before starts[0] and at or past starts[streams], tokens of no stream, are left as
+ * they are.
  * FP16 and BF16 with head_dim 64 or 128, 16-byte aligned tensors and strides, page_size a multiple
  * of 8 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
  * 256, other strides) on CUDA cores.  `workspace` holds

@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_direct_kernel(const Att
     const int head = static_cast<int>(row - token * p.args.q_heads);
     if (token >= p.args.tokens) return;
     const int b = find_stream(p.cache.starts, p.cache.streams, token);
-    if (b >= p.cache.streams) return;  // padding past the last stream
+    if (b >= p.cache.streams) return;  // no stream's
     const int d = p.cache.head_dim;
     const int kv_head = head / (p.args.q_heads / p.cache.heads);
 

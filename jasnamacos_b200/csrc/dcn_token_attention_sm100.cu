@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const int head = static_cast<int>(row - token * p.a.args.q_heads);
     const int b = row < rows ? find_stream(p.a.cache.starts, p.a.cache.streams, token) : p.a.cache.streams;
     grid_dependency_wait();
-    if (b >= p.a.cache.streams) return;  // padding past the last stream
+    if (b >= p.a.cache.streams) return;  // no stream's
     const int64_t length = p.a.cache.lengths[b];
     const Visible seen = visible_keys(length - p.a.cache.starts[b + 1] + token, length, p.a.args.window, p.a.args.sinks,
                                       p.a.args.frame);

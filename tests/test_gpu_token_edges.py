@@ -1,0 +1,87 @@
+"""GPU: calls of the token operators at the edges of what they promise, against the formulas in FP64."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import token_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, F16 = torch.float32, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from jasnamacos_b200.token_ops import CudaTokenOps
+
+    return CudaTokenOps()
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(gen, shape, dtype, scale=1.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def paged(gen, lengths, heads, dim, page, dtype):
+    """A cache of shuffled pages full of values, and the streams' table (-1 where a stream has no page)."""
+    need = [-(-n // page) for n in lengths]
+    total = sum(need) + 2
+    order = torch.randperm(total, generator=gen, device="cuda").int()
+    table = torch.full((len(lengths), max(need)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return normal(gen, (total, page, heads, dim), dtype), normal(gen, (total, page, heads, dim), dtype), table
+
+
+# ---- tokens before the first stream's ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("lead,steps,lengths", [(5, [3, 4], [40, 9]), (3000, [3500, 2600], [9000, 4000])])
+def test_append_leaves_out_tokens_before_the_first_stream(ops, dtype, lead, steps, lengths):
+    """starts may begin past 0, as a slice of a larger batch's does: the tokens before it are no stream's.  Few
+    tokens, and enough for the kernel that copies rows whole."""
+    g = generator(lead)
+    k_cache, v_cache, table = paged(g, lengths, 4, 128, 64, dtype)
+    starts = ints([lead, lead + steps[0], lead + sum(steps)])
+    k, v = (normal(g, (lead + sum(steps) + 2, 4, 128), dtype) for _ in range(2))
+    want_k, want_v = k_cache.clone(), v_cache.clone()
+    for b, n in enumerate(lengths):
+        at = torch.arange(n - steps[b], n, device="cuda")
+        page = table[b].long()[at // 64]
+        lo = int(starts[b])
+        want_k[page, at % 64], want_v[page, at % 64] = k[lo:lo + steps[b]], v[lo:lo + steps[b]]
+    ops.append(k, v, k_cache, v_cache, table, starts, ints(lengths))
+    assert torch.equal(k_cache, want_k) and torch.equal(v_cache, want_v)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("steps,lengths,split", [([1, 3], [40, 9], False), ([1, 2], [5000, 30], True),
+                                                 ([300, 2], [300, 30], False), ([300, 7], [5000, 60], True)])
+def test_attention_leaves_out_tokens_before_the_first_stream(ops, dtype, steps, lengths, split):
+    """Rows of no stream keep what the result held, whichever kernel runs and whether its keys are split."""
+    g = generator(sum(lengths))
+    k_cache, v_cache, table = paged(g, lengths, 1, 64, 64, dtype)
+    lead = 9
+    starts = ints([lead, lead + steps[0], lead + sum(steps)])
+    q = normal(g, (lead + sum(steps) + 2, 2, 64), dtype, 1.5)
+    s = dict(q=q, k_cache=k_cache, v_cache=v_cache, table=table, starts=starts, lengths=ints(lengths))
+    limits = dict(max_q=max(steps), max_kv=max(lengths), window=10000)
+    assert (ops.attention_workspace_bytes(**s, **limits) > 0) == (split and dtype == F16)
+    out = torch.full_like(q, 3.0)
+    ops.attention(**s, **limits, out=out)
+    want, bound = ref.attention(**s, window=10000)
+    end = lead + sum(steps)
+    ref.check(out[lead:end], want[lead:end], bound[lead:end])
+    assert bool((out[:lead] == 3).all()) and bool((out[end:] == 3).all())
