@@ -3,7 +3,7 @@
 //
 // For a row i of queries, over its visible keys s, in one pass with a running maximum m and sum l:
 //   S = Q K^T            tcgen05.mma, Q and K tiles in shared memory, S in tensor memory
-//   P = exp2(c S - c m)  c = scale log2 e; a thread owns a row, so maximum and sum need no exchange
+//   P = exp2(c S - c m + kRaise)  c = scale log2 e; a thread owns a row, so maximum and sum need no exchange
 //   O += P V             tcgen05.mma, P (rounded to the element type) in tensor memory
 //   out = O / l
 //
@@ -17,11 +17,15 @@
 // launch joins the parts.  Key tiles come by TMA, a box a page (or a power-of-two part of one), into a
 // ring that is filled ahead across row blocks.
 //
-// Rounding P to the element type (as its values are the second product's operand) costs a relative
-// 2^-12 (FP16) or 2^-9 (BF16) per weight, of the size of the result's own rounding; l sums the
+// Rounding P to the element type (as its values are the second product's operand) costs a weight a
+// relative 2^-11 (FP16) or 2^-8 (BF16) at most, of the size of the result's own rounding; l sums the
 // unrounded weights in FP32.  The maximum that P is taken against may lag the true one by up to
-// 2^8 before O is rescaled: exact up to the range of P (256 of FP16's 65504), and it spares almost
-// every rescaling.
+// 2^8 before O is rescaled, which spares almost every rescaling.  FP16 weights are taken 2^7 larger than
+// that, up to 2^15 of its 65504: below 2^-21 of the maximum in use they are subnormal, to an absolute 2^-32 of
+// it.  (Without, to 2^-25: of 262,143 weights of 2^-25.1 nothing was left in O, while l counted them.)
+// The tensor core adds the products to O in FP32, each cut at 2^-25 of the sum it is added to: measured, beside one
+// weight and value of 1 it keeps 97 % of FP16 weights of 2^-21.6, 73 % of 2^-24.5 and none of 2^-25.1; BF16 the same
+// within its result's rounding.
 //
 // What bounds it, measured on one B200:
 // - Four clips of 7,680 tokens (FP16, 16 query and 8 key heads of 128, a window of 9 frames of 256): 490 us,
@@ -49,6 +53,8 @@ constexpr int kTmemCols = 512;      // S0, S1 (128 each), O0, O1 (head_dim each)
 constexpr uint32_t kTmemO = 256;
 constexpr uint32_t kTmemP = 384;    // P0, P1 of head_dim 64; of 128, where there is no room, P lies over S
 constexpr float kLag = 8.0f;        // log2 of how far the maximum in use may lag
+template <typename T>
+constexpr float kRaise = __is_same(T, __half) ? 7.0f : 0.0f;  // log2 of what weights are larger by (BF16 has FP32's range)
 constexpr int kSmCount = 148;
 constexpr int64_t kMaxItems = int64_t{1} << 20;  // of a launch, where one stream's row blocks are what makes them many
 
@@ -66,7 +72,7 @@ struct Layout {
 struct KernelParams {
     AttentionParams a;
     float *part_o;       // [parts][tokens][q_heads][head_dim] unnormalised O; null: write the result
-    float2 *part_ml;     // [parts][tokens][q_heads] (c m, l)
+    float2 *part_ml;     // [parts][tokens][q_heads] (c m - kRaise, l)
     uint32_t *err;
     int ratio;           // query heads of a key head
     int per_ratio;       // 2^16 / ratio, rounded up: r * per_ratio >> 16 is r / ratio for a tile's rows
@@ -205,7 +211,7 @@ struct alignas(1024) Smem {
     // The current item of each softmax warp and of the product warp's two streams, kept here: the 128
     // scores of a row need the registers.
     Item item[kSoftmaxWarps + 2];
-    float2 other_ml[kRows];  // stream 1's (c m, l), where stream 0 merges the two
+    float2 other_ml[kRows];  // stream 1's (c m - kRaise, l), where stream 0 merges the two
     int other_dirty;         // and whether its rows are to be done alone
     int dirty[2][2];         // by the parity of an item's number: the last item whose rows are to be done alone
     int abort_flag;
@@ -863,7 +869,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                             tmem_st_32x32b_x16_wait(o_tmem + d, o);
                         }
                     }
-                    const float mc = m == -INFINITY ? 0.0f : m * p.c;
+                    const float mc = m == -INFINITY ? 0.0f : m * p.c - kRaise<T>;
                     const uint64_t c2 = pair_of(p.c, p.c), mc2 = pair_of(-mc, -mc);
                     uint64_t sum[2] = {0, 0};  // two FP32 zeros each
 #pragma unroll
@@ -908,7 +914,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             // tensor memory, whose lanes both warpgroups reach.
             const bool merge = !Shared && p.part_o == nullptr;
             float2 other = make_float2(-INFINITY, 0.0f);
-            float mc = m * p.c;
+            const float mc = m * p.c - kRaise<T>;
             if (merge && s == 1) {
                 sm.other_ml[row] = any ? make_float2(mc, l) : other;
                 if (row == 0) sm.other_dirty = alone;
@@ -1004,8 +1010,8 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
     if (warp == kSoftmaxWarps) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the parts of a row: out = sum_j 2^(M_j - M) O_j / sum_j 2^(M_j - M) l_j, M the largest of
-// the parts' maxima M_j (in log2).  One warp a row; parts in their order, so the result does not
+// Joins the parts of a row: out = sum_j 2^(M_j - M) O_j / sum_j 2^(M_j - M) l_j, M_j what the part's weights were
+// taken against (in log2), M the largest of them.  One warp a row; parts in their order, so the result does not
 // depend on which block was first.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ KernelParams p, int parts) {

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -9,7 +11,7 @@ import token_reference as ref
 
 pytestmark = pytest.mark.gpu
 
-F32, F16 = torch.float32, torch.float16
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
 
 @pytest.fixture(scope="module")
@@ -85,3 +87,33 @@ def test_attention_leaves_out_tokens_before_the_first_stream(ops, dtype, steps, 
     end = lead + sum(steps)
     ref.check(out[lead:end], want[lead:end], bound[lead:end])
     assert bool((out[:lead] == 3).all()) and bool((out[end:] == 3).all())
+
+
+# ---- FP16 weights far below the largest ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("streams,step,heads", [(1, 9472, 4), (4, 1, 37)])
+def test_attention_many_small_weights(ops, dtype, streams, step, heads):
+    """One key of weight 1, met first, whose value is 0, and 262,143 of weight 2^-25.1, whose values are 1 and make
+    up the result.  All rows see all keys, and there are enough rows that no further launch splits them.
+
+    Bound, of the result: a rounding of it and of the weights; a product's cut at 2^-25 of the sum it is added to, of
+    each key; the chain of FP32 sums, two a tile of 128 keys.  And FP16 has weights of this size in multiples of
+    2^-31: half of one, of each key."""
+    keys, dim, page = 262144, 64, 1024
+    q = torch.zeros(streams * step, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 17.40625
+    k = torch.zeros(keys // page, page, heads, dim, dtype=dtype, device="cuda")
+    k[0, 0, :, 0] = 1.0
+    v = torch.ones_like(k)
+    v[0, 0] = 0.0
+    s = dict(q=q, k_cache=k, v_cache=v, table=torch.arange(keys // page, device="cuda").int().expand(streams, -1).contiguous(),
+             starts=ints([step * b for b in range(streams + 1)]), lengths=ints([keys] * streams), max_q=step, max_kv=keys,
+             window=1, frame=1 << 20)
+    assert ops.attention_workspace_bytes(**s) == 0
+    rest = (keys - 1) * math.exp(-q[0, 0, 0].item())
+    want = rest / (rest + 1)
+    bound = want * (2 * ref.U[dtype] + keys * 2.0 ** -25 + keys / 64 * 2.0 ** -24) + (keys * 2.0 ** -32 if dtype == F16 else 0)
+    off = (ops.attention(**s, scale=1.0).double() - want).abs().max().item()
+    assert off <= bound, f"off by {off:.3g}, bound {bound:.3g}"
