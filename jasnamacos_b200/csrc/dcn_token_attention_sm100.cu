@@ -38,6 +38,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <cfloat>
 #include <mutex>
 
 #include "dcn_token_attention.cuh"
@@ -1221,9 +1222,10 @@ cudaError_t launch_token_attention_tensor(const AttentionParams &a, void *worksp
     k.splits = plan.splits;
     k.box_rows = box_rows(a.cache.page_size);
     k.items = static_cast<int>(plan.items);
-    // Above zero, so that a hidden key's score of -inf stays -inf; 1e-30 makes every weight 1 as 0 would.
+    // Above zero, so that a hidden key's score of -inf stays -inf.  The smallest normal makes every weight 1 as 0 would,
+    // to 2^-6 for products of 2^120 and to FP32's rounding below 2^102.
     const float c = fabsf(a.args.scale) * 1.4426950408889634f;
-    k.c = c > 1e-30f ? c : 1e-30f;
+    k.c = c > FLT_MIN ? c : FLT_MIN;
     k.negate = a.args.scale < 0.0f;
     CUtensorMap k_map, v_map;
     const dcn_paged_cache &cache = a.cache;

@@ -117,3 +117,19 @@ def test_attention_many_small_weights(ops, dtype, streams, step, heads):
     bound = want * (2 * ref.U[dtype] + keys * 2.0 ** -25 + keys / 64 * 2.0 ** -24) + (keys * 2.0 ** -32 if dtype == F16 else 0)
     off = (ops.attention(**s, scale=1.0).double() - want).abs().max().item()
     assert off <= bound, f"off by {off:.3g}, bound {bound:.3g}"
+
+
+# ---- scales near zero ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("steps", [[1, 2], [200, 3]])
+@pytest.mark.parametrize("scale", [2.0 ** -104, -2.0 ** -104, 0.0])
+def test_attention_small_scale_of_large_products(ops, dtype, steps, scale):
+    """Queries and keys of 2^52: their products times the scale are ordinary scores."""
+    g = generator(21)
+    k_cache, v_cache, table = paged(g, [700, 150], 2, 64, 64, dtype)
+    s = dict(q=normal(g, (sum(steps), 4, 64), dtype, 2.0 ** 51), k_cache=k_cache * 2.0 ** 52, v_cache=v_cache, table=table,
+             starts=ints([0, steps[0], sum(steps)]), lengths=ints([700, 150]))
+    want, bound = ref.attention(**s, window=400, scale=scale)
+    ref.check(ops.attention(**s, max_q=max(steps), max_kv=700, window=400, scale=scale), want, bound)
