@@ -579,7 +579,10 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                                 tc_fence_after();
                                 scores(s, r, here.slot);
                             }
-                            if ((cuts & 1u) && s == 0 && lane == 0) mbar_arrive(&sm.scan_go);
+                            // An item's first tile is asked for when both streams have begun the item: the scan marks
+                            // it where the item before the last had its mark, which stream 1 may still be about to
+                            // read, as it is not waited for over an item without rows of its own.
+                            if ((cuts & 1u) && s == (i < 0 ? 1 : 0) && lane == 0) mbar_arrive(&sm.scan_go);
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
                         }

@@ -133,3 +133,31 @@ def test_attention_small_scale_of_large_products(ops, dtype, steps, scale):
              starts=ints([0, steps[0], sum(steps)]), lengths=ints([700, 150]))
     want, bound = ref.attention(**s, window=400, scale=scale)
     ref.check(ops.attention(**s, max_q=max(steps), max_kv=700, window=400, scale=scale), want, bound)
+
+
+# ---- rows done alone, item after item --------------------------------------------------------
+
+
+def test_attention_rows_alone_beside_short_steps(ops):
+    """A block takes a step of two row tiles, one of a single tile, and again one of two, each with a value that is
+    not finite and that only the last rows see: each item's rows are done alone on its own account."""
+    n, dim = 148, 64
+    steps = [200] * n + [100] * n + [200] * n
+    lengths = [264] * (3 * n)
+    g = generator(22)
+    k_cache, v_cache, table = paged(g, lengths, 1, dim, 24, F16)
+    starts = ints([sum(steps[:b]) for b in range(3 * n + 1)])
+    s = dict(q=normal(g, (sum(steps), 1, dim), F16, 1.5), k_cache=k_cache, v_cache=v_cache, table=table, starts=starts,
+             lengths=ints(lengths))
+    want, bound = ref.attention(**s, window=10000)
+    v = v_cache.clone()
+    v[table[:, 260 // 24].long(), 260 % 24, 0, 5] = float("inf")
+    out = ops.attention(**dict(s, v_cache=v), max_q=200, max_kv=264, window=10000)
+    stream = torch.repeat_interleave(torch.arange(3 * n, device="cuda"), torch.tensor(steps, device="cuda"))
+    position = 264 - starts.long()[stream + 1] + torch.arange(sum(steps), device="cuda")
+    clean = position < 260
+    ref.check(out[clean], want[clean], bound[clean])
+    assert not bool(torch.isfinite(out[~clean][..., 5]).any())
+    other = torch.arange(dim, device="cuda") != 5
+    ref.check(out[..., other], want[..., other], bound[..., other])
+    assert ops.lib.dcn_device_error() == 0
