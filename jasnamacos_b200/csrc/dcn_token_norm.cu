@@ -304,6 +304,11 @@ token_norm_folded_kernel(const __grid_constant__ dcn_token_norm_args a, int bloc
         }
         segment = segment_end;
     }
+    if (!ok) {  // the rows under way may still land: not in another block's memory
+        static_assert(kStages == 2, "the other stage and its parity");
+        mbar_wait_bounded(&landed[warp][stage], parity, nullptr);
+        mbar_wait_bounded(&landed[warp][stage ^ 1], parity ^ static_cast<uint32_t>(stage), nullptr);
+    }
 }
 
 template <typename T, int VEC, int NT, int NV, int kTeams>

@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(kRowThreads) rotate_rows_kernel(const __grid_c
     __syncthreads();
     if (!mbar_wait_bounded(&landed, 0, nullptr)) {
         atomicOr(err, kErrWaitTimeout);
+        mbar_wait_bounded(&landed, 0, nullptr);  // the copies may still land: not in another block's memory
         return;
     }
 
