@@ -164,18 +164,17 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
 
 // ---- streams ---------------------------------------------------------------------------
 
-// The stream that holds `token`: how many of starts[1..streams] are at or below it.  Called by a
-// whole warp; returns `streams` for a token that no stream holds, past the last one's or before the
-// first one's.  One 32-wide load per 32 streams instead of a chain of dependent loads.
+// The stream that holds `token`: the last one whose start is at or below it.  Called by a whole warp;
+// returns `streams` for a token that no stream holds, past the last one's or before the first one's.
+// One 32-wide load per 32 starts instead of a chain of dependent loads.
 __device__ __forceinline__ int find_stream(const int32_t *starts, int streams, int64_t token) {
     const int lane = threadIdx.x & 31;
-    const bool before = token < starts[0];
-    int below = 0;
-    for (int b = 0; b < streams; b += 32) {
-        const bool at_or_below = b + lane < streams && starts[b + lane + 1] <= token;
-        below += __popc(__ballot_sync(0xffffffffu, at_or_below));
+    int begun = 0;  // how many of starts[0..streams] are at or below the token
+    for (int b = 0; b <= streams; b += 32) {
+        const bool at_or_below = b + lane <= streams && starts[b + lane] <= token;
+        begun += __popc(__ballot_sync(0xffffffffu, at_or_below));
     }
-    return before ? streams : below;
+    return begun > 0 ? begun - 1 : streams;
 }
 
 #endif  // __CUDACC__
