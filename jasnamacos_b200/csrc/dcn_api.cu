@@ -110,6 +110,7 @@ struct DeviceInfo {
     int sm_count = 0;
     uint32_t *err_word = nullptr;
     uint64_t ctx_id = 0;
+    bool attention_ready = false, norm_ready = false;  // the token operators' own kernels
 };
 
 std::mutex g_mutex;
@@ -151,14 +152,13 @@ dcn_status current_device(DeviceInfo **out) {
             e = fused_prepare_device(&d.err_word);
             if (e == cudaSuccess) e = slab_prepare_device();
             if (e == cudaSuccess) e = temporal_prepare_device();
-            if (e == cudaSuccess) e = token_attention_prepare_device();
-            if (e == cudaSuccess) e = token_norm_prepare_device();
             if (e != cudaSuccess) {
                 cudaGetLastError();
                 return from_cuda(e);
             }
         }
         d.ctx_id = current_context_id();
+        d.attention_ready = d.norm_ready = false;
         d.ready = true;
     }
     if (!d.sm100) return DCN_ERR_UNSUPPORTED;  // the library carries sm_100a code only
@@ -221,11 +221,25 @@ dcn_path select_path(const Params &p) {
 
 }  // namespace
 
-dcn_status launch_device(LaunchDevice *out) {
+dcn_status launch_device(LaunchDevice *out, KernelSet set) {
     DeviceInfo *d = nullptr;
     const dcn_status st = current_device(&d);
-    if (st == DCN_OK) *out = LaunchDevice{d->sm_count, d->err_word};
-    return st;
+    if (st != DCN_OK) return st;
+    if (set != KernelSet::kNone) {
+        const bool attention = set == KernelSet::kTokenAttention;
+        std::lock_guard<std::mutex> lock(g_mutex);
+        bool &ready = attention ? d->attention_ready : d->norm_ready;
+        if (!ready) {
+            const cudaError_t e = attention ? token_attention_prepare_device() : token_norm_prepare_device();
+            if (e != cudaSuccess) {
+                cudaGetLastError();
+                return from_cuda(e);
+            }
+            ready = true;
+        }
+    }
+    *out = LaunchDevice{d->sm_count, d->err_word};
+    return DCN_OK;
 }
 
 dcn_status status_from_cuda(cudaError_t e) { return from_cuda(e); }

@@ -77,7 +77,10 @@ struct LaunchDevice {
     int sm_count;
     uint32_t *err_word;
 };
-dcn_status launch_device(LaunchDevice *out);
+// Kernels that are set up by the first launch that needs them, once per device and context: a device that refuses
+// them, or a program that never launches them, has the other operators all the same.
+enum class KernelSet { kNone, kTokenAttention, kTokenNorm };
+dcn_status launch_device(LaunchDevice *out, KernelSet set = KernelSet::kNone);
 dcn_status status_from_cuda(cudaError_t e);
 
 // Longest any device-side wait may spin before it gives up and reports

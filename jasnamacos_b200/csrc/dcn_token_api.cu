@@ -185,10 +185,11 @@ dcn_status dcn_token_attention(const dcn_paged_cache *cache, const dcn_token_att
     const size_t need = dcn_token_attention_workspace_bytes(cache, args);
     if (need > 0 && (workspace == nullptr || !aligned_to(workspace, 16) || workspace_bytes < need))
         return DCN_ERR_INVALID_ARGUMENT;
+    const bool tensor = token_attention_tensor(*cache, *args) && packs(*q) && packs(*out);
     LaunchDevice dev;
-    if ((st = launch_device(&dev)) != DCN_OK) return st;
+    if ((st = launch_device(&dev, tensor ? KernelSet::kTokenAttention : KernelSet::kNone)) != DCN_OK) return st;
     AttentionParams p{*cache, *args, *q, *out};
-    if (token_attention_tensor(*cache, *args) && packs(*q) && packs(*out))
+    if (tensor)
         return status_from_cuda(launch_token_attention_tensor(p, workspace, dev.sm_count, dev.err_word,
                                                               reinterpret_cast<cudaStream_t>(stream)));
     return status_from_cuda(launch_token_attention_direct(p, reinterpret_cast<cudaStream_t>(stream)));
@@ -216,7 +217,7 @@ dcn_status dcn_token_norm(const dcn_token_norm_args *args, dcn_stream stream) {
     for (int64_t s : strides)
         if (!valid_stride(s)) return DCN_ERR_INVALID_ARGUMENT;
     LaunchDevice dev;
-    dcn_status st = launch_device(&dev);
+    const dcn_status st = launch_device(&dev, KernelSet::kTokenNorm);
     if (st != DCN_OK) return st;
     return status_from_cuda(launch_token_norm(a, dev.err_word, reinterpret_cast<cudaStream_t>(stream)));
 }

@@ -3,6 +3,10 @@
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
 
 import pytest
 import torch
@@ -12,6 +16,7 @@ import token_reference as ref
 pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+REPO = Path(__file__).resolve().parent.parent
 
 
 @pytest.fixture(scope="module")
@@ -161,3 +166,79 @@ def test_attention_rows_alone_beside_short_steps(ops):
     other = torch.arange(dim, device="cuda") != 5
     ref.check(out[..., other], want[..., other], bound[..., other])
     assert ops.lib.dcn_device_error() == 0
+
+
+# ---- set-up of one operator and the others ---------------------------------------------------
+
+
+def test_convolution_does_not_depend_on_the_token_operators(tmp_path):
+    """Where the set-up of the attention and norm kernels fails, as it would with kernels that a device refuses, those
+    operators say so and the others run.  The failure is a stand-in for the two set-up functions, loaded ahead of them."""
+    fake = tmp_path / "fake.cpp"
+    fake.write_text("namespace dcn {\nint token_attention_prepare_device() { return 9; }  // invalid configuration\n"
+                    "int token_norm_prepare_device() { return 9; }\n}\n")
+    lib = tmp_path / "libfake.so"
+    subprocess.run(["g++", "-shared", "-fPIC", "-o", str(lib), str(fake)], check=True)
+    code = f"""
+        import ctypes, sys
+        sys.path.insert(0, {str(REPO)!r})
+        ctypes.CDLL({str(lib)!r}, mode=ctypes.RTLD_GLOBAL)
+        import torch
+        from jasnamacos_b200 import synthetic
+        from jasnamacos_b200.deform_conv import CommandFailed, CudaDeformConv
+        from jasnamacos_b200.token_ops import CudaTokenOps
+        inp = synthetic.generate(1)
+        out = CudaDeformConv().run_float16(inp.shape, inp.input, inp.offset, inp.mask, inp.weight, inp.bias)
+        print("convolution", out.size)
+        ops = CudaTokenOps()
+        x = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
+        at, f = torch.zeros(4, 3, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.float64, device="cuda")
+        ops.rotary(x, at, f, (1, 0, 0))
+        print("rotary")
+        cache = torch.zeros(1, 16, 2, 64, dtype=torch.float16, device="cuda")
+        one = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+        s = dict(k_cache=cache, v_cache=cache, table=one[None, :1].contiguous(), starts=one, lengths=one[1:])
+        ops.append(x, x, **s)
+        limits = dict(max_q=4, max_kv=4, window=4)
+        ops.attention(x.float(), **dict(s, k_cache=cache.float(), v_cache=cache.float()), **limits)
+        print("attention on CUDA cores")
+        for name, call in (("attention", lambda: ops.attention(x, **s, **limits)), ("norm", lambda: ops.norm(x.view(4, 128)))):
+            for again in range(2):
+                try:
+                    call()
+                except CommandFailed:
+                    print(name, "refused")
+        torch.cuda.synchronize()
+    """
+    done = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+    said = done.stdout.split("\n")
+    assert said[1:-1] == ["rotary", "attention on CUDA cores"] + ["attention refused"] * 2 + ["norm refused"] * 2, done.stdout
+
+
+def test_first_call_of_an_operator_may_be_captured():
+    """In a process that has launched other operators: the set-up of attention and norm is no stream operation."""
+    code = f"""
+        import sys
+        sys.path.insert(0, {str(REPO)!r})
+        import torch
+        from jasnamacos_b200.token_ops import CudaTokenOps
+        ops = CudaTokenOps()
+        x = torch.randn(512, 2, 64, device="cuda").half()
+        at, f = torch.zeros(512, 3, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.float64, device="cuda")
+        ops.rotary(x, at, f, (1, 0, 0))
+        cache = torch.randn(1, 512, 2, 64, device="cuda").half()
+        one = torch.tensor([0, 512], dtype=torch.int32, device="cuda")
+        s = dict(k_cache=cache, v_cache=cache, table=one[None, :1].contiguous(), starts=one, lengths=one[1:])
+        rows = torch.randn(9001, 512, device="cuda").half()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a = ops.attention(x, **s, max_q=512, max_kv=512, window=512)
+            n = ops.norm(rows)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ops.attention(x, **s, max_q=512, max_kv=512, window=512)) and torch.equal(n, ops.norm(rows))
+        assert bool(a.isfinite().all()) and bool(n.isfinite().all()) and bool(n.any())
+    """
+    done = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
