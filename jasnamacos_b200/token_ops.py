@@ -29,6 +29,9 @@ from .deform_conv import DeviceUnavailable, InvalidArgument, raise_for_status
 _DTYPES = {torch.float32: _native.DCN_DTYPE_F32, torch.float16: _native.DCN_DTYPE_F16,
            torch.bfloat16: _native.DCN_DTYPE_BF16}
 _KINDS = {"rms": _native.DCN_NORM_RMS, "layer": _native.DCN_NORM_LAYER}
+# ctypes keeps an integer's low bits only: the heads and widths of a larger tensor go in as this, which the library
+# refuses.
+_MOST = (1 << 31) - 1
 
 
 def _said(name, t, wanted) -> InvalidArgument:
@@ -115,6 +118,8 @@ class CudaTokenOps:
             raise _said("table", table, f"a [streams, columns] int32 tensor on {self.device}")
         pages, page_size, heads, head_dim = shape
         streams, columns = table.shape
+        if (pages | page_size | heads | head_dim | streams | columns) > _MOST:
+            raise InvalidArgument(f"k_cache {tuple(shape)}, table {tuple(table.shape)}: 32-bit sizes are wanted")
         table_stride, unit = table.stride()
         if unit != 1 and columns > 1:
             raise _said("table", table, "unit stride along its rows")
@@ -135,6 +140,8 @@ class CudaTokenOps:
             raise InvalidArgument(f"x is {tuple(x.shape)}; [tokens, heads, head_dim] is wanted")
         shape = x.shape
         tokens, heads, head_dim = shape
+        if heads > _MOST or head_dim > _MOST:
+            heads = head_dim = _MOST
         x_at = self._tokens("x", x, shape, x.dtype)
         rotation = self._rotation(positions, frequencies, pairs, interleaved, tokens)
         if out is None:
@@ -176,17 +183,17 @@ class CudaTokenOps:
             q_out_at = self._tokens("q_out", q_out, q_shape, dtype)
         elif q_out is not None:
             raise InvalidArgument("q_out needs q")
-        self._call(stream, self.lib.dcn_token_append, cache, tokens, rotation, k_at, v_at, q_heads, q_at,
-                   q_out_at)
+        self._call(stream, self.lib.dcn_token_append, cache, tokens, rotation, k_at, v_at,
+                   q_heads if q_heads <= _MOST else _MOST, q_at, q_out_at)
         return q_out
 
     # -- attention ---------------------------------------------------------------
     def _attention_args(self, tokens, q_heads, max_q, max_kv, window, sinks, frame, scale):
-        # ctypes keeps an integer's low bits only.
-        if max(max_q, max_kv, window, sinks, frame) >= 1 << 31 or min(max_q, max_kv, window, sinks, frame) < 0:
+        if not 0 <= (max_q | max_kv | window | sinks | frame) <= _MOST:
             raise InvalidArgument(f"max_q {max_q}, max_kv {max_kv}, window {window}, sinks {sinks}, frame {frame}: "
                                   "32-bit counts are wanted")
-        return _native.DcnTokenAttentionArgs(tokens, q_heads, max_q, max_kv, window, sinks, frame, scale, 0)
+        return _native.DcnTokenAttentionArgs(tokens, q_heads if q_heads <= _MOST else _MOST, max_q, max_kv, window, sinks, frame,
+                                             scale, 0)
 
     def attention(self, q, k_cache, v_cache, table, starts, lengths, max_q, max_kv, window, sinks=0, frame=1, scale=None,
                   out=None, workspace=None, stream=None):
@@ -279,7 +286,7 @@ class CudaTokenOps:
         scale_at, scale_stride = self._modulation("scale", scale, groups, width, dtype)
         shift_at, shift_stride = self._modulation("shift", shift, groups, width, dtype)
         args = _native.DcnTokenNormArgs(
-            rows, group, width, self._dtype(x), _KINDS[kind], post, eps, residual_scale, x_at, residual_at,
+            rows, group, width if width <= _MOST else _MOST, self._dtype(x), _KINDS[kind], post, eps, residual_scale, x_at, residual_at,
             self._vector("post_weight", post_weight, width, dtype), self._vector("post_bias", post_bias, width, dtype),
             self._vector("weight", weight, width, dtype), self._vector("bias", bias, width, dtype), gate_at, scale_at, shift_at,
             hidden_at, out_at, x_stride, residual_stride, hidden_stride, out_stride, gate_stride, scale_stride, shift_stride)

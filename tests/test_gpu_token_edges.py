@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import token_reference as ref
+from jasnamacos_b200.deform_conv import InvalidArgument, InvalidShape, Unsupported
 
 pytestmark = pytest.mark.gpu
 
@@ -166,6 +167,37 @@ def test_attention_rows_alone_beside_short_steps(ops):
     other = torch.arange(dim, device="cuda") != 5
     ref.check(out[..., other], want[..., other], bound[..., other])
     assert ops.lib.dcn_device_error() == 0
+
+
+# ---- sizes past 32 bits ----------------------------------------------------------------------
+
+
+def test_sizes_past_32_bits_are_refused(ops):
+    """Refused, not cut to their low bits: here 64 elements of a row, one head, one page."""
+    wide = torch.zeros(1, 2 ** 32 + 64, dtype=F16, device="cuda")
+    with pytest.raises(Unsupported):
+        ops.norm(wide, out=wide)
+    with pytest.raises(Unsupported):
+        ops.residual_norm(wide, wide, hidden=wide, out=wide)
+    x = wide[:, :64].view(1, 1, 64).expand(1, 2 ** 32 + 1, 64)
+    at, f = torch.zeros(1, 3, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.float64, device="cuda")
+    with pytest.raises(InvalidShape):
+        ops.rotary(x, at, f, (1, 0, 0), out=x)
+    cache = torch.zeros(1, 16, 1, 64, dtype=F16, device="cuda")
+    many_pages = cache.expand(2 ** 32 + 1, 16, 1, 64)
+    long_page = cache[:, :1].expand(1, 2 ** 32 + 1, 1, 64)
+    row = torch.zeros(1, 1, 64, dtype=F16, device="cuda")
+    for pages in (many_pages, long_page):
+        s = dict(k_cache=pages, v_cache=pages, table=ints([[0]]), starts=ints([0, 1]), lengths=ints([1]))
+        with pytest.raises(InvalidArgument):
+            ops.append(row, row, **s)
+        with pytest.raises(InvalidArgument):
+            ops.attention(row, **s, max_q=1, max_kv=1, window=1)
+    s = dict(k_cache=cache, v_cache=cache, table=ints([[0]]), starts=ints([0, 1]), lengths=ints([1]))
+    with pytest.raises(InvalidShape):
+        ops.append(row, row, **s, q=x, q_out=x)
+    with pytest.raises(InvalidShape):
+        ops.attention(x, **s, max_q=1, max_kv=1, window=1, out=x)
 
 
 # ---- set-up of one operator and the others ---------------------------------------------------
