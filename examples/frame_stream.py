@@ -3,7 +3,8 @@
 Per frame and stream: the DCN aligns the tile's features (64 channels, 64x64), they are cut into
 4x4 patches (256 tokens of 1,024 values), and a block attends from them to the last `window` frames
 and the first `sinks` frames of the stream.  The frames live in a paged cache, one frame a page; pages
-of frames that left the window are used again, so a stream may run on for good.
+of frames that left the window are used again, and so are their positions, so a stream may run on for
+good (its time positions are 32-bit: two years at 30 frames a second).
 
     python examples/frame_stream.py --streams 8 --frames 30
 
@@ -60,15 +61,16 @@ class Weights:
 class FrameStream:
     """The block's state for `streams` streams that take frames together."""
 
-    def __init__(self, weights: Weights, streams: int, window: int = 8, sinks: int = 1, most_frames: int = 1024):
+    def __init__(self, weights: Weights, streams: int, window: int = 8, sinks: int = 1):
         self.ops = CudaTokenOps()
         self.w, self.streams, self.window, self.sinks = weights, streams, window, sinks
         self.frame = 0
         pages = sinks + window  # of a stream
         self.k_cache = torch.zeros(streams * pages, TOKENS, KV_HEADS, HEAD_DIM, dtype=torch.float16, device="cuda")
         self.v_cache = torch.zeros_like(self.k_cache)
-        # Frame f's page: the first frames keep theirs, the others take turns.
-        f = torch.arange(most_frames, device="cuda")
+        # Frame f's page: the first frames keep theirs, the others take turns.  Frames from sinks + window on see the
+        # first frames and a whole window behind them, so their places in the stream repeat with their pages.
+        f = torch.arange(sinks + 2 * window, device="cuda")
         page = torch.where(f < sinks, f, sinks + (f - sinks) % window)
         self.table = (page + pages * torch.arange(streams, device="cuda")[:, None]).int().contiguous()
         self.starts = (TOKENS * torch.arange(streams + 1, device="cuda")).int()
@@ -83,9 +85,12 @@ class FrameStream:
         """One frame of every stream: tokens [streams * TOKENS, WIDTH] FP16 in and out."""
         ops, w = self.ops, self.w
         shift1, scale1, gate1, shift2, scale2, gate2 = w.modulation.unbind(1)
+        place = self.frame
+        if place >= self.sinks + self.window:
+            place = self.sinks + self.window + (place - self.sinks) % self.window
         self.positions[:, 0] = self.frame
         self.frame += 1
-        self.lengths += TOKENS
+        self.lengths.fill_((place + 1) * TOKENS)
 
         x = ops.norm(tokens, kind="layer", weight=w.norm1, scale=scale1, shift=shift1, group=TOKENS)
         qkv = (x @ w.qkv).view(-1, HEADS + 2 * KV_HEADS, HEAD_DIM)
@@ -93,7 +98,7 @@ class FrameStream:
         q = ops.append(k, v, self.k_cache, self.v_cache, self.table, self.starts, self.lengths, q=q, positions=self.positions,
                        frequencies=self.frequencies, pairs=PAIRS)
         attended = ops.attention(q, self.k_cache, self.v_cache, self.table, self.starts, self.lengths, max_q=TOKENS,
-                                 max_kv=self.frame * TOKENS, window=self.window, sinks=self.sinks, frame=TOKENS)
+                                 max_kv=(place + 1) * TOKENS, window=self.window, sinks=self.sinks, frame=TOKENS)
         tokens, x = ops.residual_norm(attended.view(-1, HEADS * HEAD_DIM) @ w.out, tokens, gate=gate1, kind="layer",
                                       weight=w.norm2, scale=scale2, shift=shift2, group=TOKENS)
         x = torch.nn.functional.silu(x @ w.up) @ w.down

@@ -67,3 +67,39 @@ def test_example_runs_behind_the_convolution(example, monkeypatch, capsys):
     monkeypatch.setattr("sys.argv", ["frame_stream.py", "--streams", "2", "--frames", "3"])
     example.main()
     assert "finite: True" in capsys.readouterr().out
+
+
+def test_stream_runs_on_for_good(example):
+    """Past 1,024 frames of one stream, where a table with a column a frame would have to end.  Bound: as above."""
+    window, sinks, last = 2, 1, 1030
+    w = example.Weights.random(1, seed=4)
+    block = example.FrameStream(w, 1, window=window, sinks=sinks)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    tokens, heads, kv, dim = example.TOKENS, example.HEADS, example.KV_HEADS, example.HEAD_DIM
+    shift1, scale1, gate1, shift2, scale2, gate2 = (m.double() for m in w.modulation.unbind(1))
+    frames = torch.randn(16, tokens, example.WIDTH, generator=g, device="cuda").half()
+    keys, values = {}, {}
+    for f in range(last):
+        x = frames[f % 16]
+        got = block.step(x)
+        if sinks <= f < 1020:
+            continue
+        y = ref.normalised(x.double(), "layer", 1e-6)[0] * w.norm1.double() * (1 + scale1) + shift1
+        qkv = (y @ w.qkv.double()).view(-1, heads + 2 * kv, dim)
+        positions = block.positions.clone()
+        positions[:, 0] = f
+        qk = ref.rotary(qkv[:, :heads + kv].float(), positions, block.frequencies, example.PAIRS, False)[0]
+        keys[f], values[f] = qk[:, heads:], qkv[:, heads + kv:]
+        if f < 1022:
+            continue
+        seen = [i for i in keys if i < sinks or i > f - window]
+        k = torch.cat([keys[i] for i in seen]).repeat_interleave(heads // kv, 1)
+        v = torch.cat([values[i] for i in seen]).repeat_interleave(heads // kv, 1)
+        p = torch.softmax(torch.einsum("qhd,khd->hqk", qk[:, :heads], k) * dim ** -0.5, -1)
+        attended = torch.einsum("hqk,khd->qhd", p, v).reshape(-1, heads * dim) @ w.out.double()
+        hidden = x.double() + gate1 * attended
+        n = ref.normalised(hidden, "layer", 1e-6)[0] * w.norm2.double() * (1 + scale2) + shift2
+        want = hidden + gate2 * (torch.nn.functional.silu(n @ w.up.double()) @ w.down.double())
+        off = ((got.double() - want).norm() / want.norm()).item()
+        assert off <= 6e-3, (f, off)
+    assert block.ops.lib.dcn_device_error() == 0
