@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import token_reference as ref
+from jasnamacos_b200 import _native
 from jasnamacos_b200.deform_conv import InvalidArgument, InvalidShape, Unsupported
 
 pytestmark = pytest.mark.gpu
@@ -274,3 +275,109 @@ def test_first_call_of_an_operator_may_be_captured():
     """
     done = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---- keys without a page ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("steps", [[1, 2, 1], [300, 3, 200], [33, 3, 40]])
+@pytest.mark.parametrize("spoiled", [False, True])
+def test_attention_keys_without_a_page_are_zeros(ops, dtype, steps, spoiled):
+    """Visible positions whose page id is outside the cache, or that lie past the table, have a key and a value of
+    zeros; also for rows that are done alone beside a value that is not finite."""
+    g = generator(23)
+    lengths, page = [900, 130, 500], 64
+    k_cache, v_cache, table = paged(g, lengths, 2, 64, page, dtype)
+    pages = k_cache.shape[0]
+    table[0, 3], table[0, 7], table[1, 0], table[2, 2] = -1, pages, -(2 ** 31), 2 ** 31 - 1
+    cut = table[:, :12].contiguous()  # stream 0 runs on for 132 positions more
+    s = dict(q=normal(g, (sum(steps), 4, 64), dtype, 1.5), k_cache=k_cache, v_cache=v_cache, table=cut,
+             starts=ints([0, steps[0], steps[0] + steps[1], sum(steps)]), lengths=ints(lengths))
+    full = torch.full((3, 15), pages, dtype=torch.int32, device="cuda")  # the reference has a page of zeros there
+    full[:, :12] = torch.where((cut >= 0) & (cut < pages), cut, pages)
+    zeros = torch.zeros_like(k_cache[:1])
+    t = dict(s, k_cache=torch.cat([k_cache, zeros]), v_cache=torch.cat([v_cache, zeros]), table=full)
+    want, bound = ref.attention(**t, window=600, sinks=70)
+    clean = torch.ones(sum(steps), dtype=torch.bool, device="cuda")
+    if spoiled:
+        at = 497  # of stream 2, which only the rows from it on see
+        s["v_cache"] = v_cache.clone()
+        s["v_cache"][table[2, at // page].long(), at % page, :, 7] = float("nan")
+        clean[steps[0] + steps[1]:] = torch.arange(500 - steps[2], 500, device="cuda") < at
+    out = ops.attention(**s, max_q=max(steps), max_kv=900, window=600, sinks=70)
+    ref.check(out[clean], want[clean], bound[clean])
+    assert bool(out[~clean][..., 7].isnan().all())
+    other = torch.arange(64, device="cuda") != 7
+    ref.check(out[..., other], want[..., other], bound[..., other])
+
+
+# ---- a caller's own scratch ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("steps", [[1], [300]])
+def test_attention_workspace_of_the_caller(ops, steps):
+    g = generator(24)
+    k_cache, v_cache, table = paged(g, [5000], 2, 64, 64, F16)
+    s = dict(q=normal(g, (steps[0], 4, 64), F16, 1.5), k_cache=k_cache, v_cache=v_cache, table=table, starts=ints([0, steps[0]]),
+             lengths=ints([5000]))
+    want, bound = ref.attention(**s, window=10000)
+    limits = dict(max_q=steps[0], max_kv=5000, window=10000)
+    need = ops.attention_workspace_bytes(**s, **limits)
+    assert need > 0
+    guarded = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = ops.attention(**s, **limits, workspace=guarded[:need])
+    ref.check(out, want, bound)
+    assert bool((guarded[need:] == 0xA5).all())
+    kept = out.clone()
+    for bad in (guarded[:need - 16], guarded[1:need + 1], guarded[:0], guarded[::2], torch.zeros(need, dtype=torch.uint8)):
+        with pytest.raises(InvalidArgument):
+            ops.attention(**s, **limits, workspace=bad, out=out)
+    assert torch.equal(out, kept)
+    three = dict(s, q=s["q"][:, :3])  # three query heads over two key heads
+    with pytest.raises(InvalidShape):
+        ops.attention(**three, **limits)
+
+
+def test_attention_on_two_streams_at_once(ops):
+    """One object, two CUDA streams, calls that split their keys: each has its own scratch."""
+    g = generator(25)
+    k_cache, v_cache, table = paged(g, [20000, 9000], 2, 128, 64, BF16)
+    calls = []
+    for seed in range(2):
+        s = dict(q=normal(g, (2, 8, 128), BF16, 1.5), k_cache=k_cache, v_cache=v_cache, table=table, starts=ints([0, 1, 2]),
+                 lengths=ints([20000, 9000]), max_q=1, max_kv=20000, window=30000)
+        assert ops.attention_workspace_bytes(**s) > 0
+        calls.append((s, ops.attention(**s)))
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(50):
+        for i, side in enumerate(sides):
+            got[i].append(ops.attention(**calls[i][0], stream=side))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, calls[i][1]) for o in got[i])
+
+
+# ---- results that a caller leaves out ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows,width,post", [(3, 1155, False), (40, 1024, True), (9001, 512, False), (9001, 512, True)])
+def test_norm_with_one_result(ops, dtype, rows, width, post):
+    """The C entry with hidden alone and with out alone: the same bits as with both."""
+    g = generator(rows + width)
+    x, residual = normal(g, (rows, width), dtype), normal(g, (rows, width), dtype)
+    weight = 1 + normal(g, (width,), dtype, 0.1)
+    hidden, out = ops.residual_norm(x, residual, post_weight=weight if post else None, residual_scale=0.5)
+    for keep in ("hidden", "out"):
+        result = torch.full_like(x, 3.0)
+        at = weight.data_ptr() if post else None
+        args = _native.DcnTokenNormArgs(
+            rows=rows, group=rows, width=width, dtype=_native.DCN_DTYPE_F32 if dtype == F32 else _native.DCN_DTYPE_F16,
+            kind=_native.DCN_NORM_RMS, post=int(post), epsilon=1e-6, residual_scale=0.5, x=x.data_ptr(),
+            residual=residual.data_ptr(), post_weight=at, x_stride=width, residual_stride=width, hidden_stride=width,
+            out_stride=width, **{keep: result.data_ptr()})
+        assert ops.lib.dcn_token_norm(args, torch.cuda.current_stream().cuda_stream or None) == _native.DCN_OK
+        assert torch.equal(result, hidden if keep == "hidden" else out)
