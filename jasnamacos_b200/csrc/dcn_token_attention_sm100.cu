@@ -483,7 +483,11 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
             };
             Walk<Shared> walk0(0), walk1(1);
             const Item *item = sm.item + kSoftmaxWarps;
-            while (ok) {
+            // Whether stream 1 may still be at the item before the last: it is not waited for over an item without rows
+            // of its own.  An item's first tile is then asked to be looked through when it has begun that item too, as
+            // the mark goes where the item before the last had its own, which stream 1 has yet to read.
+            bool behind = false;
+            for (; ok; behind = !item[1].rows()) {
                 {
                     Item next[2];
                     if (!walk0.next(p, next[0]) || !walk1.next(p, next[1])) break;
@@ -579,10 +583,7 @@ attention_kernel(const __grid_constant__ KernelParams p, const __grid_constant__
                                 tc_fence_after();
                                 scores(s, r, here.slot);
                             }
-                            // An item's first tile is asked for when both streams have begun the item: the scan marks
-                            // it where the item before the last had its mark, which stream 1 may still be about to
-                            // read, as it is not waited for over an item without rows of its own.
-                            if ((cuts & 1u) && s == (i < 0 ? 1 : 0) && lane == 0) mbar_arrive(&sm.scan_go);
+                            if ((cuts & 1u) && s == (i < 0 && behind ? 1 : 0) && lane == 0) mbar_arrive(&sm.scan_go);
                             if (release) umma_commit_if(issue, &sm.empty[r][here.slot]);
                             here.advance();
                         }
