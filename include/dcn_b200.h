@@ -433,8 +433,9 @@ dcn_status dcn_forward_f16_static_scratch(const dcn_shape *shape, const void *in
  *
  * Tensors may be strided: a token tensor is [tokens][heads][head_dim] with the strides of dcn_heads
  * (in elements) and unit stride along head_dim.  A token count of zero is a valid call that
- * launches nothing; a tensor has at most 4096 heads.  Arithmetic is FP32 whatever the element type,
- * rounded once per output. */
+ * launches nothing; a tensor has at most 4096 heads.  Sums, statistics and the arithmetic between them are
+ * FP32 whatever the element type, angles FP64; results are rounded once.  Attention on the tensor cores also
+ * rounds each weight to the element type, as an operand of its product with the values. */
 
 /* A strided [tokens][heads][head_dim] tensor (strides in elements, non-negative). */
 typedef struct dcn_heads {
@@ -513,8 +514,11 @@ dcn_status dcn_token_append(const dcn_paged_cache *cache, int64_t tokens, const 
  * they are.
  * FP16 and BF16 with head_dim 64 or 128, 16-byte aligned tensors and strides, page_size a multiple
  * of 8 and q_heads / heads <= 128 run on the tensor cores; everything else (FP32, other head_dim up to
- * 256, other strides) on CUDA cores.  `workspace` holds
- * dcn_token_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0). */
+ * 256, other strides and page sizes) on CUDA cores, some hundred to a thousand times slower in long steps.
+ * On the tensor cores a weight is rounded to the element type (FP16: to 2^-32 of the largest at least), and a
+ * product that is below 2^-25 of the sum it is added to is lost; on CUDA cores all is FP32.
+ * `workspace` holds dcn_token_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0).  It
+ * is the call's own until its work on the stream has ended: calls that may run at the same time need one each. */
 typedef struct dcn_token_attention_args {
     int64_t tokens; /* rows of q and out */
     int32_t q_heads;

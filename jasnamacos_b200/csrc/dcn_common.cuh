@@ -84,7 +84,8 @@ dcn_status launch_device(LaunchDevice *out, KernelSet set = KernelSet::kNone);
 dcn_status status_from_cuda(cudaError_t e);
 
 // Longest any device-side wait may spin before it gives up and reports
-// DCN_ERR_DEVICE_TIMEOUT (nanoseconds of %globaltimer).
+// DCN_ERR_DEVICE_TIMEOUT (nanoseconds of %globaltimer).  Attention over the paged cache begins a wait anew while
+// another of the block's warps gets on with rows that it does one by one, whose work is finite.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 // Bits of the sticky device error word.

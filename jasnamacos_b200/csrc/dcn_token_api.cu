@@ -7,7 +7,7 @@ using namespace dcn;
 
 namespace {
 
-constexpr int64_t kMaxStride = int64_t{1} << 40;  // elements; every offset then fits 63 bits
+constexpr int64_t kMaxStride = int64_t{1} << 40;  // elements; offsets inside an allocation then fit 63 bits
 constexpr int32_t kMaxHeads = 4096;  // of one tensor
 
 size_t element_bytes(int dtype) { return dtype == DCN_DTYPE_F32 ? 4 : 2; }

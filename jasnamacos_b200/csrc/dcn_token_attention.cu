@@ -1,9 +1,9 @@
 // dcn_token_attention.cu -- attention over a paged cache with a sliding window of frames and first
 // frames that stay visible, on CUDA cores: every type, head_dim up to 256, any strides.
 //
-// One warp computes one row, 32 keys at a time (RowByWarp).  It reads each key once per row and feeds no
-// tensor core, so it is bound by issue (four clips of 7,680 tokens: 487 ms); the shapes that matter take the
-// tensor-core kernel.
+// One warp computes one row, 32 keys at a time (RowByWarp).  Each lane reads a key of its own element by element,
+// no key is shared between rows, and nothing goes to the tensor cores: four clips of 7,680 tokens take 487 ms here.
+// The shapes that matter take the tensor-core kernel.
 #include "dcn_token_attention.cuh"
 
 namespace dcn {

@@ -27,14 +27,16 @@
 // weight and value of 1 it keeps 97 % of FP16 weights of 2^-21.6, 73 % of 2^-24.5 and none of 2^-25.1; BF16 the same
 // within its result's rounding.
 //
-// What bounds it, measured on one B200:
-// - Four clips of 7,680 tokens (FP16, 16 query and 8 key heads of 128, a window of 9 frames of 256): 490 us,
-//   1,026 TFLOP/s.  A pair of tiles takes some 3,600 cycles; 3,072 of them the tensor core's, as a product
-//   with both operands in shared memory takes twice its arithmetic for their reads.
-// - Eight streams' frames of 256 tokens, head_dim 64: 50 us; 3,280 cycles a pair of tiles, the softmax warps'
-//   own latency, with the exponentials' 2,048 in it.
-// - 64 streams of one token over 4,160 keys (BF16, 32 and 8 heads of 128): 172 us, 5.98 TB/s, memory.
-// - Four streams of one token over up to 260 keys: 12.9 us, a chain of steps whose code each runs once.
+// What bounds it, measured on one B200, a short burst of calls in a graph (in brackets one call of many back to
+// back, where the 1 kW limit lowers the clock):
+// - Four clips of 7,680 tokens (FP16, 16 query and 8 key heads of 128, a window of 8 frames of 256 and one that
+//   stays): 490 to 497 us, 1,010 to 1,026 TFLOP/s (573 us, 877).  A pair of tiles takes some 3,600 cycles.  Its products
+//   are 2,048 of them (512 for 128x128x128, measured alike with both operands in shared memory and with one in
+//   tensor memory) and its exponentials 2,048 as well: neither unit is full, the two streams overlap in part.
+// - Eight streams' frames of 256 tokens, head_dim 64: 50 us (51); 3,280 cycles a pair of tiles, 2,048 of them
+//   exponentials, 1,024 products; the rest is the softmax warps' latency in this layout of two a scheduler.
+// - 64 streams of one token over 4,160 keys (BF16, 32 and 8 heads of 128): 172 us, 5.98 TB/s (197, 5.2), memory.
+// - Four streams of one token over up to 260 keys: 13.1 us, a chain of steps whose code each runs once.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1121,7 +1123,7 @@ Plan make_plan(const dcn_paged_cache &c, const dcn_token_attention_args &a) {
     // Split the keys of a row block over as many blocks as make the whole shortest: rounds of the
     // GPU's blocks, each as long as its tiles plus a fixed part (start, queries, result), plus the join.  Both parts are
     // three tiles' time: with a join for nothing, 1,944 tokens of 2 heads over 29 of their keys were split and took 25.0 us
-    // where unsplit they take 20.8; with one of a tile, or a start of one, 15 drawn calls stayed within 4 %.
+    // where unsplit they take 20.8.  Neither figure is a sharp one.
     const int streams = plan.shared ? 1 : 2;
     int64_t best = INT64_MAX;
     plan.splits = 1;
